@@ -49,7 +49,7 @@ extern "C" {
  * Q3_K = 11 are the public ggml ids the reference table lacks). */
 enum {
     WM_F32 = 0, WM_F16 = 1, WM_Q8_0 = 8, WM_Q2_K = 10, WM_Q3_K = 11,
-    WM_Q4_K = 12, WM_Q5_K = 13, WM_Q6_K = 14
+    WM_Q4_K = 12, WM_Q5_K = 13, WM_Q6_K = 14, WM_BF16 = 30
 };
 
 /* Workspace status bits (read back with wm_workspace_status). */
@@ -265,6 +265,104 @@ int wm_expert_ffn(const void* gate, int gate_type, const void* up, int up_type, 
                   int down_type, const float* x, int H, int I, float* out, void* ws, int64_t ws_bytes,
                   void* stream);
 int64_t wm_expert_workspace_size(int H, int I);
+
+/* ----------------------------------------------- operators on 16-bit weights */
+/* The products of an expert layer whose weights are held as fp16 or bf16 (GGUF
+ * tensors of type F16 and BF16, or a layer in training), for any number of
+ * rows from one token to a whole batch, with their gradients.  The reference
+ * has no such path (its experts are quantised and it does not train).
+ *
+ * All matrices are row-major with their last dimension contiguous; every ld is
+ * the distance of two rows in elements.  Pointers need only the alignment of
+ * their type and sizes may be odd; rows that begin at multiples of 16 bytes
+ * are read fastest.  Products and sums are kept in fp32 and each output is
+ * rounded once (to nearest even), when it is stored.  Outputs must not overlap
+ * inputs, except that residual may be y itself (same ld and type).
+ *
+ * Groups: rows offsets[e] <= r < offsets[e + 1] belong to expert e (device
+ * int32 [n_groups + 1], not decreasing; wm_group_by_expert makes them).  Groups
+ * may be empty.  Rows before the first and behind the last group are neither
+ * read nor written.  Offsets outside [0, rows] are taken as the nearer bound,
+ * so no memory outside the rows is touched whatever they hold. */
+#define WM_ACT_NONE 0
+#define WM_ACT_RELU 1
+#define WM_ACT_SILU 2
+#define WM_ACT_GELU 3    /* z * Phi(z), exact */
+#define WM_ACT_SWIGLU 4  /* silu(gate) * up; W holds the gate rows, then the up rows */
+typedef struct wm_product_desc {
+    int32_t dtype;           /* WM_F16 or WM_BF16: x, w, bias, residual, pre, dz, dx */
+    int32_t rows;            /* rows of the product (0: nothing to do) */
+    int32_t in;              /* columns of x and w */
+    int32_t out;             /* rows of one w; with WM_ACT_SWIGLU twice the columns of y */
+    int32_t n_groups;        /* experts; 1 when offsets is NULL */
+    int32_t x_rows;          /* rows that x has */
+    int32_t act;             /* WM_ACT_* */
+    int32_t y_type;          /* type of y: dtype or WM_F32 */
+    const int32_t* offsets;  /* device [n_groups + 1], or NULL: all rows are one group */
+    const int32_t* token;    /* device [rows]: the row of x that row r takes (outside [0, x_rows): zeros),
+                                or NULL: row r itself */
+    const void* x;           /* [x_rows][in] */
+    int64_t ldx;
+    const void* w;           /* [n_groups][out][in] */
+    int64_t ldw;
+    int64_t w_stride;        /* elements between experts */
+    const void* bias;        /* [n_groups][out] dense, or NULL */
+    const void* residual;    /* [rows][columns of y], or NULL */
+    int64_t ld_residual;
+    void* y;                 /* [rows][out, or out / 2 with WM_ACT_SWIGLU] */
+    int64_t ldy;
+    void* pre;               /* [rows][out]: receives x W^T + bias before the activation, or NULL */
+    int64_t ld_pre;
+} wm_product_desc;
+
+/* Bytes of workspace a call may use (0: none; < 0: bad descriptor).  backward:
+ * 0 for wm_product, 1 for wm_product_backward.  One call at a time may use a
+ * workspace; it needs no clearing and keeps nothing between calls. */
+int64_t wm_product_workspace_size(const wm_product_desc* d, int backward);
+
+/* y[r] = act(W_e x[token[r]] + bias_e) + residual[r] for every row r of every
+ * group e. */
+int wm_product(const wm_product_desc* d, void* ws, int64_t ws_bytes, void* stream);
+
+/* Gradients of z = x W^T + bias, given dz [rows][out] (dtype):
+ *   dx[r] = W_e^T dz[r]             [rows][in] (dtype), one row per row of dz: with
+ *                                   token, wm_combine_rows sums them per row of x
+ *   dw[e] = sum_r dz[r] x[token[r]]^T  [n_groups][out][in] dense, dw_type dtype or WM_F32
+ *   db[e] = sum_r dz[r]             [n_groups][out] fp32
+ * Any of dx, dw, db may be NULL.  dw and db of an empty group are zeros.  The
+ * sums run in a fixed order: the same call gives the same bits.  d->y, bias,
+ * residual and pre are not used and d->act must be WM_ACT_NONE (see
+ * wm_act_backward for the step before). */
+int wm_product_backward(const wm_product_desc* d, const void* dz, int64_t ld_dz, void* dx, int64_t ld_dx, void* dw,
+                        int dw_type, float* db, void* ws, int64_t ws_bytes, void* stream);
+
+/* dz = act'(pre) * dy: dy [rows][cols], pre and dz [rows][cols] or, with
+ * WM_ACT_SWIGLU, [rows][2 cols] (gate half, up half).  dz may be pre. */
+int wm_act_backward(int dtype, int act, int64_t rows, int cols, const void* dy, int64_t ld_dy, const void* pre,
+                    int64_t ld_pre, void* dz, int64_t ld_dz, void* stream);
+
+/* Sorts T * K picks by expert, stably: ids int32 [T][K] (device).  offsets
+ * [E + 1]; token [T * K]: the token of each sorted row; row [T][K]: the sorted
+ * row of each pick.  A pick outside [0, E) belongs to no expert: its row is -1,
+ * and token is -1 from offsets[E] on.  T * K < 2^31 - 2^16. */
+int wm_group_by_expert(const int32_t* ids, int T, int K, int E, int32_t* offsets, int32_t* token, int32_t* row,
+                       void* stream);
+
+/* out[t] = sum_k w[t][k] * y[row[t][k]] + residual[t], k in order: y [rows][H]
+ * (dtype), row int32 [T][K], w fp32 [T][K] or NULL (ones), residual and out
+ * [T][H] of out_type (dtype or WM_F32), residual NULL or out itself.  A row
+ * outside [0, rows) adds nothing, whatever its weight. */
+int wm_combine_rows(int dtype, const void* y, int64_t ld_y, int rows, const int32_t* row, const float* w, int T, int K,
+                    int H, const void* residual, int64_t ld_residual, void* out, int64_t ld_out, int out_type,
+                    void* stream);
+
+/* Its gradients, given dout [T][H] (dout_type: dtype or WM_F32): dy[row[t][k]]
+ * = w[t][k] * dout[t] (dtype; rows that no pick names are left as they are)
+ * and dw[t][k] = <dout[t], y[row[t][k]]> (fp32; 0 where the row is outside
+ * [0, rows)).  dy or dw may be NULL; a row may be named by one pick only. */
+int wm_combine_rows_backward(int dtype, const void* dout, int64_t ld_dout, int dout_type, const void* y, int64_t ld_y,
+                             int rows, const int32_t* row, const float* w, int T, int K, int H, void* dy,
+                             int64_t ld_dy, float* dw, void* stream);
 
 /* ------------------------------------------------- decode without allocation */
 /* No counterpart in the reference: for callers that cannot allocate device

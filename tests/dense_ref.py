@@ -1,0 +1,81 @@
+"""Plain 64-bit forms of the 16-bit operators and the error bounds their tests
+use (not collected).
+
+Bounds.  A product's fp32 sum of n exact terms, in any order, is off by at most
+(n - 1) 2^-24 sum|terms| (1 + small); the bounds here take (n + 2) 2^-23, twice
+that, for matrix instructions that cut instead of rounding inside.  An
+activation with slope at most L passes an error on L times; its own evaluation
+adds a few 2^-24 of its value (16 are allowed, the functions used are good to
+a few).  Storing rounds by at most eps / 2 of the stored value, or half a step
+of the smallest one."""
+import math
+
+import torch
+
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}
+SLOPE = {"none": 1.0, "relu": 1.0, "silu": 1.1, "gelu": 1.13}
+
+
+def rounding(v, dtype):
+    """Largest error of storing values of magnitude up to |v|."""
+    return torch.finfo(dtype).eps / 2 * v + TINY[dtype]
+
+
+def act(z, name):
+    if name == "swiglu":
+        g, u = z.chunk(2, 1)
+        return g * torch.sigmoid(g) * u
+    if name == "silu":
+        return z * torch.sigmoid(z)
+    if name == "gelu":
+        return 0.5 * z * torch.special.erfc(-z * math.sqrt(0.5))
+    return torch.relu(z) if name == "relu" else z            # slope 0 at 0
+
+
+def act_grad(dy, z, name):
+    z = z.detach().clone().requires_grad_(True)
+    act(z, name).backward(dy)
+    return z.grad
+
+
+def product(x, w, bias, name, dtype):
+    """(z, bound of z, y, bound of y before rounding) of act(x w^T + bias) for one group."""
+    x, w = x.double().cpu(), w.double().cpu()
+    z, mag = x @ w.T, x.abs() @ w.abs().T
+    if bias is not None:
+        z, mag = z + bias.double().cpu(), mag + bias.double().cpu().abs()
+    dz = (x.shape[1] + 2) * 2.0 ** -23 * mag
+    y = act(z, name)
+    if name == "swiglu":
+        (g, u), (dg, du) = z.chunk(2, 1), dz.chunk(2, 1)
+        dy = 1.1 * dg * (u.abs() + du) + (g * torch.sigmoid(g)).abs() * du
+    else:
+        dy = SLOPE[name] * dz
+    return z, dz, y, dy + 16 * 2.0 ** -24 * y.abs()
+
+
+def within(got, want, bound, what=""):
+    """|got - want| <= bound + the rounding of got's type, everywhere."""
+    got64 = got.detach().double().cpu()
+    lim = bound + rounding(want.abs() + bound, got.dtype)
+    err = (got64 - want).abs()
+    bad = ~(err <= lim)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside; worst {float((err / lim).max()):.2f} bounds"
+
+
+def grouping(ids, E):
+    """(offsets, token, row) by a loop over the picks."""
+    T, K = ids.shape
+    rows = [[] for _ in range(E)]
+    for t in range(T):
+        for k in range(K):
+            if 0 <= int(ids[t, k]) < E:
+                rows[int(ids[t, k])].append((t, k))
+    offsets, token, row = [0], [], torch.full((T, K), -1, dtype=torch.int32)
+    for r in rows:
+        for t, k in r:
+            row[t, k] = len(token)
+            token.append(t)
+        offsets.append(len(token))
+    token += [-1] * (T * K - len(token))
+    return torch.tensor(offsets, dtype=torch.int32), torch.tensor(token, dtype=torch.int32), row

@@ -1,0 +1,125 @@
+"""Refusals of the 16-bit operators and their empty calls, without a GPU: the C
+entry points check before they touch a device, the Python functions before they
+call them."""
+import ctypes as C
+
+import pytest
+import torch
+
+from dense_ref import grouping
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from winmoe_amd import _lib
+    return _lib.load()
+
+
+def desc(**kw):
+    """A sound product of 4 rows, 16 x 8 weights, at made-up addresses that no check follows."""
+    from winmoe_amd import _lib
+    d = _lib.ProductDesc()
+    d.dtype, d.rows, d.inn, d.out, d.n_groups, d.x_rows, d.y_type = _lib.BF16, 4, 8, 16, 1, 4, _lib.BF16
+    d.x, d.w, d.y = 4096, 8192, 16384
+    d.ldx, d.ldw, d.ldy = 8, 8, 16
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+BAD = [dict(dtype=0), dict(dtype=8), dict(rows=-1), dict(rows=(1 << 30) + 1), dict(inn=0), dict(out=0),
+       dict(inn=(1 << 26) + 1), dict(n_groups=0), dict(n_groups=2), dict(n_groups=(1 << 16) + 1, offsets=64),
+       dict(offsets=66), dict(token=65), dict(x_rows=3), dict(x_rows=-1, token=64), dict(ldx=7), dict(ldw=7),
+       dict(n_groups=2, offsets=64, w_stride=127), dict(act=-1), dict(act=5), dict(x=None), dict(w=None), dict(y=None),
+       dict(x=4097), dict(w=8193), dict(y=16385), dict(y_type=1), dict(y_type=0, y=16386), dict(ldy=15),
+       dict(bias=65), dict(residual=65, ld_residual=16), dict(residual=64, ld_residual=15), dict(pre=64, ld_pre=15),
+       dict(pre=65, ld_pre=16), dict(act=4, out=15), dict(act=4, ldy=7)]
+
+
+@pytest.mark.parametrize("kw", BAD, ids=str)
+def test_product_refuses(lib, kw):
+    assert lib.wm_product(C.byref(desc(**kw)), None, 0, None) == -2
+
+
+@pytest.mark.parametrize("kw", [b for b in BAD if set(b) <= {"dtype", "rows", "inn", "n_groups", "ldx", "ldw", "x_rows"}], ids=str)
+def test_product_workspace_and_backward_refuse(lib, kw):
+    d = desc(**kw)
+    assert lib.wm_product_workspace_size(C.byref(d), 0) < 0
+    assert lib.wm_product_backward(C.byref(d), 64, 16, 64, 8, None, 0, None, None, 0, None) == -2
+
+
+def test_product_backward_refuses(lib):
+    d = desc()
+    call = lambda d, dz=64, ldz=16, dx=None, ldx=8, dw=None, wt=30, db=None: lib.wm_product_backward(
+        C.byref(d), dz, ldz, dx, ldx, dw, wt, db, None, 0, None)
+    assert call(desc(act=1), dx=64) == -2                    # the activation's gradient is a step of its own
+    assert call(d, dz=None, dx=64) == -2
+    assert call(d, dz=65, dx=64) == -2
+    assert call(d, ldz=15, dx=64) == -2
+    assert call(d, dx=65) == -2
+    assert call(d, dx=64, ldx=7) == -2
+    assert call(desc(w=None), dx=64) == -2
+    assert call(desc(x=None), dw=64) == -2
+    assert call(d, dw=64, wt=1) == -2                        # fp16 gradients of bf16 weights
+    assert call(d, dw=66, wt=0) == -2
+    assert call(d, db=66) == -2
+    assert lib.wm_product(None, None, 0, None) == -2
+
+
+def test_pair_operators_refuse(lib):
+    bf, f32 = 30, 0
+    assert lib.wm_act_backward(f32, 1, 4, 8, 64, 8, 64, 8, 64, 8, None) == -2
+    assert lib.wm_act_backward(bf, 7, 4, 8, 64, 8, 64, 8, 64, 8, None) == -2
+    assert lib.wm_act_backward(bf, 4, 4, 8, 64, 8, 64, 8, 64, 16, None) == -2       # pre must be twice as wide
+    assert lib.wm_act_backward(bf, 1, 4, 0, 64, 8, 64, 8, 64, 8, None) == -2
+    assert lib.wm_act_backward(bf, 1, -1, 8, 64, 8, 64, 8, 64, 8, None) == -2
+    assert lib.wm_act_backward(bf, 1, 4, 8, None, 8, 64, 8, 64, 8, None) == -2
+    g = lib.wm_group_by_expert
+    assert g(64, 1, 0, 4, 64, 64, 64, None) == -2
+    assert g(64, 1, 1, 0, 64, 64, 64, None) == -2
+    assert g(64, 1 << 20, 1 << 11, 4, 64, 64, 64, None) == -2
+    assert g(64, 1, 1, 4, None, 64, 64, None) == -2
+    assert g(None, 1, 1, 4, 64, 64, 64, None) == -2
+    assert g(66, 1, 1, 4, 64, 64, 64, None) == -2
+    c = lib.wm_combine_rows
+    assert c(f32, 64, 8, 4, 64, 64, 2, 2, 8, None, 0, 64, 8, f32, None) == -2
+    assert c(bf, 64, 8, 4, 64, 64, 2, 2, 8, None, 0, 64, 8, 1, None) == -2
+    assert c(bf, 64, 7, 4, 64, 64, 2, 2, 8, None, 0, 64, 8, bf, None) == -2
+    assert c(bf, 64, 8, 4, 64, 64, 2, 2, 8, 64, 7, 64, 8, bf, None) == -2
+    assert c(bf, 64, 8, 4, None, 64, 2, 2, 8, None, 0, 64, 8, bf, None) == -2
+    assert c(bf, 64, 8, 4, 64, 64, 2, 2, 8, None, 0, 66, 8, f32, None) == -2
+    b = lib.wm_combine_rows_backward
+    assert b(bf, 64, 8, 1, 64, 8, 4, 64, 64, 2, 2, 8, 64, 8, None, None) == -2
+    assert b(bf, 64, 7, bf, 64, 8, 4, 64, 64, 2, 2, 8, 64, 8, None, None) == -2
+    assert b(bf, 64, 8, bf, None, 8, 4, 64, 64, 2, 2, 8, None, 8, 64, None) == -2
+    assert b(bf, 64, 8, bf, 64, 8, 4, 64, 64, 2, 2, 8, 64, 7, None, None) == -2
+
+
+def test_empty_calls_return_at_once(lib):
+    """No rows, no tokens or nothing asked for: 0, before any device is needed."""
+    assert lib.wm_product(C.byref(desc(rows=0, x=None, w=None, y=None)), None, 0, None) == 0
+    assert lib.wm_act_backward(30, 1, 0, 8, None, 0, None, 0, None, 0, None) == 0
+    assert lib.wm_combine_rows(30, None, 0, 0, None, None, 0, 2, 8, None, 0, None, 0, 30, None) == 0
+    assert lib.wm_combine_rows_backward(30, 64, 8, 30, 64, 8, 4, 64, 64, 2, 2, 8, None, 8, None, None) == 0
+
+
+def test_descriptor_is_as_long_as_the_headers(lib):
+    from winmoe_amd import _lib
+    assert C.sizeof(_lib.ProductDesc) == 8 * 4 + 14 * 8
+
+
+def test_python_refuses_host_tensors():
+    from winmoe_amd import dense
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    for call in (lambda: dense.linear(x, x), lambda: dense.group_by_expert(torch.zeros(2, 2, dtype=torch.int32), 4),
+                 lambda: dense.act_backward(x, x, "silu"), lambda: dense.combine(x, torch.zeros(2, 2, dtype=torch.int32)),
+                 lambda: dense.grouped_matmul(x, x.view(1, 4, 8), torch.zeros(2, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="HIP"):
+            call()
+
+
+def test_reference_grouping():
+    """The tests' own sorting, on a case small enough to see."""
+    off, token, row = grouping(torch.tensor([[2, 0], [-1, 2], [0, 3]]), 3)
+    assert off.tolist() == [0, 2, 2, 4] and token.tolist() == [0, 2, 0, 1, -1, -1]
+    assert row.tolist() == [[2, 0], [-1, 3], [1, -1]]

@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(PKG, "libwinmoe_hip.so")
 
 WM_OK, WM_ERR, WM_EINVAL = 0, -1, -2
 F32, F16, Q8_0, Q2_K, Q3_K, Q4_K, Q5_K, Q6_K = 0, 1, 8, 10, 11, 12, 13, 14
+BF16 = 30
 TYPE_NAMES = {F32: "F32", F16: "F16", Q8_0: "Q8_0", Q2_K: "Q2_K", Q3_K: "Q3_K", Q4_K: "Q4_K", Q5_K: "Q5_K",
               Q6_K: "Q6_K"}
 TYPE_IDS = {v: k for k, v in TYPE_NAMES.items()}
@@ -32,6 +33,8 @@ FLAG_SPIN_PROBE = 16
 FLAG_PREFILL_PASS16 = 32
 FLAG_PREFILL_PASS32 = 64
 
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "swiglu": 4}
+
 _vp, _i64 = C.c_void_p, C.c_int64
 
 
@@ -46,6 +49,18 @@ class LayerDesc(C.Structure):
         ("gate_stride", _i64), ("up_stride", _i64), ("down_stride", _i64),
         ("sh_gate", _vp), ("sh_up", _vp), ("sh_down", _vp), ("sh_gate_inp", _vp),
         ("norm_w", _vp), ("norm_eps", C.c_float), ("add_residual", C.c_int32),
+    ]
+
+
+class ProductDesc(C.Structure):
+    """Mirror of ``wm_product_desc``."""
+    _fields_ = [
+        ("dtype", C.c_int32), ("rows", C.c_int32), ("inn", C.c_int32), ("out", C.c_int32),
+        ("n_groups", C.c_int32), ("x_rows", C.c_int32), ("act", C.c_int32), ("y_type", C.c_int32),
+        ("offsets", _vp), ("token", _vp),
+        ("x", _vp), ("ldx", _i64), ("w", _vp), ("ldw", _i64), ("w_stride", _i64),
+        ("bias", _vp), ("residual", _vp), ("ld_residual", _i64),
+        ("y", _vp), ("ldy", _i64), ("pre", _vp), ("ld_pre", _i64),
     ]
 
 
@@ -96,6 +111,16 @@ SIGNATURES = {
     "wm_expert_ffn": (C.c_int, [_vp, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp, _i64,
                                 _vp]),
     "wm_expert_workspace_size": (_i64, [C.c_int, C.c_int]),
+    "wm_product_workspace_size": (_i64, [C.POINTER(ProductDesc), C.c_int]),
+    "wm_product": (C.c_int, [C.POINTER(ProductDesc), _vp, _i64, _vp]),
+    "wm_product_backward": (C.c_int, [C.POINTER(ProductDesc), _vp, _i64, _vp, _i64, _vp, C.c_int, _vp, _vp, _i64,
+                                      _vp]),
+    "wm_act_backward": (C.c_int, [C.c_int, C.c_int, _i64, C.c_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "wm_group_by_expert": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp]),
+    "wm_combine_rows": (C.c_int, [C.c_int, _vp, _i64, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _i64, _vp,
+                                  _i64, C.c_int, _vp]),
+    "wm_combine_rows_backward": (C.c_int, [C.c_int, _vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, _vp, C.c_int,
+                                           C.c_int, C.c_int, _vp, _i64, _vp, _vp]),
     "wm_profile_enable": (C.c_int, [C.c_int]),
     "wm_profile_read": (C.c_int, [C.POINTER(C.c_double), C.POINTER(_i64), C.c_int]),
     "wm_profile_phase_name": (C.c_char_p, [C.c_int]),
