@@ -70,50 +70,6 @@ int launch_group(const int32_t* ids, int T, int K, int E, int32_t* offsets, int3
     return (int)hipGetLastError();
 }
 
-// ------------------------------------------------------------------ 8 values at a time
-
-// 8 values at p, of which the first n exist, as fp32; no alignment needed.
-template <bool BF> WM_DEV void get8(const uint16_t* p, int n, float* v) {
-    uint16_t e[8];
-    if (n >= 8) {
-        __builtin_memcpy(e, p, 16);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) e[i] = i < n ? p[i] : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = from16<BF>(e[i]);
-}
-template <bool BF> WM_DEV void put8(uint16_t* p, int n, const float* v) {
-    uint16_t e[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) e[i] = to16<BF>(v[i]);
-    if (n >= 8) {
-        __builtin_memcpy(p, e, 16);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < n) p[i] = e[i];
-    }
-}
-WM_DEV void getf8(const float* p, int n, float* v) {
-    if (n >= 8) {
-        __builtin_memcpy(v, p, 32);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < n ? p[i] : 0.0f;
-    }
-}
-WM_DEV void putf8(float* p, int n, const float* v) {
-    if (n >= 8) {
-        __builtin_memcpy(p, v, 32);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < n) p[i] = v[i];
-    }
-}
-
 // ------------------------------------------------------------------ activation
 
 // dz = act'(pre) * dy; SwiGLU's pre and dz hold the gate half, then the up

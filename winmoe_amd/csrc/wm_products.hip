@@ -95,6 +95,19 @@ WM_DEV GroupTile find_tile(const int32_t* __restrict__ offsets, int E, int rows,
     return g;
 }
 
+// Workgroup -> tile.  Workgroups go round the 8 XCDs, so each XCD takes a
+// contiguous run of tiles, in blocks of 8 row tiles times all column tiles:
+// what runs on an XCD at once shares rows and columns in its L2.
+struct TileId {
+    int p, q;
+};
+WM_DEV TileId tile_id(int block, int blocks, int nP) {
+    const int per = blocks / 8, rest = blocks % 8, xcd = block % 8;
+    const int t = xcd * per + min(xcd, rest) + block / 8;
+    const int q8 = t / (8 * nP), nq = min(8, blocks / nP - 8 * q8), in = t - q8 * 8 * nP;
+    return {in / nq, 8 * q8 + in % nq};
+}
+
 // ------------------------------------------------------------------ LDS tiles
 
 // [TILE][64], memory rows along the contraction.  Slot s (16 bytes) holds
@@ -134,54 +147,102 @@ template <int TILE> struct AcrossC {
 
 // ------------------------------------------------------------------ epilogue
 
-template <bool BF> WM_DEV void store4(void* base, int64_t at, int f32, bool vec, int n, f32x4 v) {
-    if (f32) {
-        float* p = (float*)base + at;
-        if (vec && n >= 4) *(f32x4*)p = v;
-        else
+// A wave's FP x FQ fragments go through LDS, PH parts one after another, so
+// that a lane then holds 8 consecutive outputs of one row: one 16-byte store
+// (and bias or residual load) per row and lane instead of two of 8 bytes that
+// jump between rows, and the epilogue's code once instead of once per
+// fragment.  LDS rows are 4 floats longer than the fragments': the 16 rows
+// that a store touches fall on different banks.
+template <int FP, int FQ, int PH> constexpr int epilogue_floats() { return FQ / PH * 16 * (FP * 16 + 4); }
+
+// Outputs from p0 on (contiguous) of rows from q0 on, below qn.  lds: the wave's own.
+template <bool BF, int DIR, int FP, int FQ, int PH>
+WM_DEV void store_tile(const ProductArgs& a, int e, int p0, int q0, int qn, int outs, int lane, const f32x4 (&acc)[FP][FQ],
+                       lf32_t* lds) {
+    constexpr int ROW = FP * 16 + 4;
+    typedef __attribute__((address_space(3))) f32x4 lf32x4;
+    const bool gated = DIR == FWD && a.act == WM_ACT_SWIGLU;
+    const int units = gated ? FP : 2 * FP;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (i < n) p[i] = v[i];
-    } else {
-        uint16_t* p = (uint16_t*)base + at;
-        if (vec && n >= 4) {
-            *(uint2*)p = (uint2){to16<BF>(v[0]) | (uint32_t)to16<BF>(v[1]) << 16, to16<BF>(v[2]) | (uint32_t)to16<BF>(v[3]) << 16};
-        } else {
+    for (int ph = 0; ph < PH; ph++) {
+        wave_lds_sync();
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (i < n) p[i] = to16<BF>(v[i]);
+        for (int j = 0; j < FQ / PH; j++)
+#pragma unroll
+            for (int i = 0; i < FP; i++)
+                *(lf32x4*)(lds + (16 * j + (lane & 15)) * ROW + 16 * i + 4 * (lane >> 4)) = acc[i][ph * (FQ / PH) + j];
+        wave_lds_sync();
+#pragma unroll 1
+        for (int k = lane; k < FQ / PH * 16 * units; k += 64) {
+            const int r = k / units, u = k % units, q = q0 + ph * (FQ / PH) * 16 + r, p = p0 + 8 * u, n = outs - p;
+            if (q >= qn || n <= 0) continue;
+            // SwiGLU: 16 gate values, then the up values of the same outputs
+            const lf32_t* src = lds + r * ROW + (gated ? 32 * (u >> 1) + 8 * (u & 1) : 8 * u);
+            float z[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) z[i] = src[i];
+            if constexpr (DIR == FWD) {
+                float up[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8];
+                if (gated)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) up[i] = src[16 + i];
+                if (a.bias) {
+                    const uint16_t* b = a.bias + (int64_t)e * a.out + p;
+                    get8<BF>(b, n, v);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) z[i] += v[i];
+                    if (gated) {
+                        get8<BF>(b + outs, n, v);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) up[i] += v[i];
+                    }
+                }
+                if (a.pre) {
+                    uint16_t* pre = a.pre + (int64_t)q * a.ldpre + p;
+                    put8<BF>(pre, n, z);
+                    if (gated) put8<BF>(pre + outs, n, up);
+                }
+                if (a.act != WM_ACT_NONE)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) z[i] = act_value(a.act, z[i], up[i]);
+                if (a.res) {
+                    get8<BF>(a.res + (int64_t)q * a.ldres + p, n, v);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) z[i] += v[i];
+                }
+                if (a.y_f32) putf8((float*)a.y + (int64_t)q * a.ldy + p, n, z);
+                else put8<BF>((uint16_t*)a.y + (int64_t)q * a.ldy + p, n, z);
+            } else if constexpr (DIR == DX) {
+                put8<BF>(a.dx + (int64_t)q * a.lddx + p, n, z);
+            } else {
+                const int64_t at = ((int64_t)e * a.out + q) * a.in + p;
+                if (a.dw_f32) putf8((float*)a.dw + at, n, z);
+                else put8<BF>((uint16_t*)a.dw + at, n, z);
+            }
         }
     }
 }
 
-template <bool BF> WM_DEV f32x4 load4(const uint16_t* p, int n) {
-    f32x4 v;
+// Sum of an operand's 8 values of one column, added to s.
+template <bool BF> WM_DEV float add8(s16x8 v, float s) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = i < n ? from16<BF>(p[i]) : 0.0f;
-    return v;
+    for (int i = 0; i < 8; i++) s += from16<BF>((uint16_t)v[i]);
+    return s;
 }
 
-// z (and for SwiGLU the up half u) of outputs [p, p + 4) of row q.
-template <bool BF> WM_DEV void store_forward(const ProductArgs& a, int e, int q, int p, int outs, bool vec, f32x4 z, f32x4 u) {
-    const int n = outs - p;
-    if (n <= 0) return;
-    const bool gated = a.act == WM_ACT_SWIGLU;
-    if (a.bias) {
-        const uint16_t* b = a.bias + (int64_t)e * a.out;
-        z += load4<BF>(b + p, n);
-        if (gated) u += load4<BF>(b + outs + p, n);
-    }
-    if (a.pre) {
-        store4<BF>(a.pre, (int64_t)q * a.ldpre + p, 0, false, n, z);
-        if (gated) store4<BF>(a.pre, (int64_t)q * a.ldpre + outs + p, 0, false, n, u);
-    }
+// db of the wave's columns: lane l summed the steps of its quarter for column l % 16.
+template <int FQ> WM_DEV void store_db(const ProductArgs& a, int e, int q0, int lane, const float (&sum)[FQ]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) z[i] = act_value(a.act, z[i], u[i]);
-    if (a.res) z += load4<BF>((const uint16_t*)a.res + (int64_t)q * a.ldres + p, n);
-    store4<BF>(a.y, (int64_t)q * a.ldy + p, a.y_f32, vec, n, z);
+    for (int j = 0; j < FQ; j++) {
+        float s = sum[j];
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        const int q = q0 + 16 * j + lane;
+        if (lane < 16 && q < a.out) a.db[(int64_t)e * a.out + q] = s;
+    }
 }
 
-// ------------------------------------------------------------------ the tile kernel
+// ------------------------------------------------------------------ tile kernel for any alignment
 
 // WP x WQ waves, each a (BP / WP) x (BQ / WQ) part of the tile.  Two LDS
 // buffers: the chunks of the next 64 steps are loaded into registers while
@@ -193,7 +254,8 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     using PT = typename std::conditional<PC, AlongC<BP>, AcrossC<BP>>::type;
     using QT = typename std::conditional<QC, AlongC<BQ>, AcrossC<BQ>>::type;
     constexpr int PS = BP * 8, QS = BQ * 8, NP = (PS + NT - 1) / NT, NQ = (QS + NT - 1) / NT;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2][(BP + BQ) * 2 * BK];
+    constexpr int STAGE = (BP + BQ) * 2 * BK, PH = 1, EPI = WP * WQ * 4 * epilogue_floats<FP, FQ, PH>();
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE > EPI ? 2 * STAGE : EPI];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wp = wave % WP, wq = wave / WP;
@@ -276,23 +338,22 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     auto stage = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NP; i++)
-            if (PS % NT == 0 || tid + i * NT < PS) *(uint4*)(lds[b] + 16 * (tid + i * NT)) = pv[i];
+            if (PS % NT == 0 || tid + i * NT < PS) *(uint4*)(lds + b * STAGE + 16 * (tid + i * NT)) = pv[i];
 #pragma unroll
         for (int i = 0; i < NQ; i++)
-            if (QS % NT == 0 || tid + i * NT < QS) *(uint4*)(lds[b] + 16 * (PS + tid + i * NT)) = qv[i];
+            if (QS % NT == 0 || tid + i * NT < QS) *(uint4*)(lds + b * STAGE + 16 * (PS + tid + i * NT)) = qv[i];
     };
 
-    f32x4 acc[FP][FQ], accb[FQ];
+    f32x4 acc[FP][FQ];
+    float sum[FQ];
 #pragma unroll
     for (int i = 0; i < FP; i++)
 #pragma unroll
         for (int j = 0; j < FQ; j++) acc[i][j] = (f32x4)0.0f;
 #pragma unroll
-    for (int j = 0; j < FQ; j++) accb[j] = (f32x4)0.0f;
-    // db: one more p operand, all ones, in the first tile of p
+    for (int j = 0; j < FQ; j++) sum[j] = 0.0f;
+    // db: the first tile of p sums the operand that it reads anyway
     const bool sums = DIR == DW && a.db && p0 == 0 && wp == 0;
-    const short one = BF ? 0x3F80 : 0x3C00;
-    const s16x8 ones = {one, one, one, one, one, one, one, one};
 
     if (c0 < cn) {
         load(c0);
@@ -303,7 +364,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     for (int c = c0; c < cn; c += BK, b ^= 1) {
         const bool more = c + BK < cn;
         if (more) load(c + BK);
-        const lds8_t* pt = (const lds8_t*)lds[b];
+        const lds8_t* pt = (const lds8_t*)lds + b * STAGE;
         const lds8_t* qt = pt + BP * 2 * BK;
 #pragma unroll
         for (int ks = 0; ks < BK / 32; ks++) {
@@ -318,46 +379,204 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
                 for (int j = 0; j < FQ; j++) acc[i][j] = mfma<BF>(pf[i], qf[j], acc[i][j]);
             if (sums)
 #pragma unroll
-                for (int j = 0; j < FQ; j++) accb[j] = mfma<BF>(ones, qf[j], accb[j]);
+                for (int j = 0; j < FQ; j++) sum[j] = add8<BF>(qf[j], sum[j]);
         }
         if (more) stage(b ^ 1);
         __syncthreads();
     }
 
-    const int pl = 4 * (lane >> 4);
+    if (sums) store_db<FQ>(a, e, q0 + wq * (BQ / WQ), lane, sum);
+    if (DIR == DW && !a.dw) return;
+    store_tile<BF, DIR, FP, FQ, PH>(a, e, p0 + (gated ? wp * (BP / WP / 2) : wp * (BP / WP)), q0 + wq * (BQ / WQ), qn, outs, lane, acc,
+                                    (lf32_t*)lds + wave * epilogue_floats<FP, FQ, PH>());
+}
+
+// ------------------------------------------------------------------ tile kernel for whole 16-byte chunks
+
+// 16 bytes per lane from src to dst (the wave's, lane order).  In assembly, as
+// the compiler would wait for every such load before any later LDS read; the
+// kernel waits itself (WM_WAIT_VMCNT) before the barrier that hands a stage over.
+WM_DEV void lds_dma16(const void* src, lds8_t* dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"((uint32_t)(uintptr_t)dst), "v"(src) : "memory");
+}
+
+// Read in place of chunks that do not exist.
+static __device__ __attribute__((aligned(16))) uint16_t zero_chunk[8];
+
+// The same tile with LDS-DMA: two stages of 64 contraction steps, filled while
+// the other one is used.  The operands of a half stage (32 steps) are read
+// into registers while the products of the half before run, across the stage
+// boundary too: at the middle of stage k every wave waits for its part of
+// stage k + 1 and its last reads of stage k, and after the barrier fills stage
+// k + 2 into the buffer just left.  One barrier per stage.
+//
+// Every chunk of 8 values exists whole or not at all (operand_rules()); rows
+// and columns past the matrix repeat valid ones, as their results are not
+// stored, and steps past the end of the contraction are zeros in both operands.
+template <bool BF, int DIR, int BP, int BQ, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs a) {
+    constexpr int NT = 64 * WP * WQ, FP = BP / WP / 16, FQ = BQ / WQ / 16;
+    constexpr bool PC = DIR == FWD, QC = DIR != DW;
+    using PT = typename std::conditional<PC, AlongC<BP>, AcrossC<BP>>::type;
+    using QT = typename std::conditional<QC, AlongC<BQ>, AcrossC<BQ>>::type;
+    constexpr int PS = BP * 8, QS = BQ * 8, NP = PS / NT, NQ = QS / NT, STAGE = (BP + BQ) * 2 * BK;
+    static_assert(PS % NT == 0 && QS % NT == 0, "whole chunks per thread");
+    constexpr int PH = WP * WQ * 4 * epilogue_floats<FP, FQ, 1>() > 160 * 1024 ? 2 : 1, EPI = WP * WQ * 4 * epilogue_floats<FP, FQ, PH>();
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE > EPI ? 2 * STAGE : EPI];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wp = wave % WP, wq = wave / WP;
+    const bool gated = DIR == FWD && a.act == WM_ACT_SWIGLU;
+    const int outs = DIR == FWD ? (gated ? a.out / 2 : a.out) : a.in;
+    const int cols = gated ? BP / 2 : BP;
+    const int nP = (outs + cols - 1) / cols;
+    const TileId id = tile_id(blockIdx.x, gridDim.x, nP);
+    const int p0 = id.p * cols;
+    int e, q0, qn, c0 = 0, cn;
+    const uint16_t* w = nullptr;
+    if (DIR == DW) {
+        const int nQ = (a.out + BQ - 1) / BQ;
+        e = id.q / nQ;
+        q0 = (id.q % nQ) * BQ;
+        qn = a.out;
+        c0 = a.offsets ? min(max(a.offsets[e], 0), a.rows) : 0;
+        cn = a.offsets ? min(max(a.offsets[e + 1], c0), a.rows) : a.rows;
+    } else {
+        const GroupTile g = find_tile(a.offsets, a.E, a.rows, BQ, id.q);
+        if (g.e < 0) return;
+        e = g.e;
+        q0 = g.start + g.tile * BQ;
+        qn = g.start + g.n;
+        cn = DIR == FWD ? a.in : a.out;
+        w = a.w + (int64_t)e * a.w_stride;
+    }
+
+    // AlongC: src = the chunk's row at its column, lim = where the row ends.
+    // AcrossC: src = column of row 0, pc = the chunk's row in the stage.
+    const uint16_t *psrc[NP], *qsrc[NQ];
+    int pc[NP], qc[NQ], plim[NP], qlim[NQ];
 #pragma unroll
-    for (int j = 0; j < FQ; j++) {
-        const int q = q0 + wq * (BQ / WQ) + 16 * j + (lane & 15);
-        if (q >= qn) continue;
-        if (DIR == FWD) {
-            const bool vec = a.y_f32 ? (a.ldy % 4 == 0 && (uintptr_t)a.y % 16 == 0) : (a.ldy % 4 == 0 && (uintptr_t)a.y % 8 == 0);
-            if (gated) {
-#pragma unroll
-                for (int i = 0; i + 1 < FP; i += 2)
-                    store_forward<BF>(a, e, q, p0 + wp * (BP / WP / 2) + 8 * i + pl, outs, vec, acc[i][j], acc[i + 1][j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < FP; i++)
-                    store_forward<BF>(a, e, q, p0 + wp * (BP / WP) + 16 * i + pl, outs, vec, acc[i][j], acc[i][j]);
-            }
-        } else if (DIR == DX) {
-            const bool vec = a.lddx % 4 == 0 && (uintptr_t)a.dx % 8 == 0;
-#pragma unroll
-            for (int i = 0; i < FP; i++) {
-                const int p = p0 + wp * (BP / WP) + 16 * i + pl;
-                store4<BF>(a.dx, (int64_t)q * a.lddx + p, 0, vec, outs - p, acc[i][j]);
-            }
+    for (int i = 0; i < NP; i++) {
+        int ix;
+        PT::slot(tid + i * NT, ix, pc[i]);
+        plim[i] = cn;
+        if (PC) {
+            const int o = min(gated ? p0 + (ix >> 5) * 16 + (ix & 15) : p0 + ix, outs - 1);
+            psrc[i] = w + (int64_t)(gated && (ix & 16) ? outs + o : o) * a.ldw;
         } else {
-            const bool vec = a.in % 4 == 0 && (uintptr_t)a.dw % 16 == 0;
-            const int64_t at = ((int64_t)e * a.out + q) * a.in;
-#pragma unroll
-            for (int i = 0; i < FP; i++) {
-                const int p = p0 + wp * (BP / WP) + 16 * i + pl;
-                if (a.dw) store4<BF>(a.dw, at + p, a.dw_f32, vec, outs - p, acc[i][j]);
-            }
-            if (sums && lane < 16) a.db[(int64_t)e * a.out + q] = accb[j][0];
+            const int o = p0 + ix < outs ? p0 + ix : p0;
+            psrc[i] = (DIR == DW ? a.x : w) + o;
         }
     }
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        int ix;
+        QT::slot(tid + i * NT, ix, qc[i]);
+        qlim[i] = cn;
+        if (QC) {
+            const int r = min(q0 + ix, qn - 1);
+            if (DIR == FWD) {
+                const int t = a.token ? a.token[r] : r;
+                const bool live = (uint32_t)t < (uint32_t)a.x_rows;
+                qlim[i] = live ? cn : 0;
+                qsrc[i] = a.x + (int64_t)(live ? t : 0) * a.ldx;
+            } else {
+                qsrc[i] = a.dz + (int64_t)r * a.lddz;
+            }
+        } else {
+            qsrc[i] = a.dz + (q0 + ix < qn ? q0 + ix : q0);
+        }
+    }
+    // DW gathers rows of x: the tokens of a stage are loaded one stage ahead
+    int tok[NP];
+    auto tokens = [&](int c) __attribute__((always_inline)) {
+        if (DIR == DW && a.token)
+#pragma unroll
+            for (int i = 0; i < NP; i++) tok[i] = c + pc[i] < cn ? a.token[c + pc[i]] : -1;
+    };
+    auto fill = [&](int c, int b) __attribute__((always_inline)) {
+        lds8_t* dst = (lds8_t*)lds + b * STAGE + 1024 * wave;
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int at = c + pc[i];
+            const uint16_t* src;
+            if (PC) {
+                src = at < plim[i] ? psrc[i] + at : zero_chunk;
+            } else if (DIR == DW) {
+                const int t = a.token ? tok[i] : at;
+                src = at < cn && (uint32_t)t < (uint32_t)a.x_rows ? psrc[i] + (int64_t)t * a.ldx : zero_chunk;
+            } else {
+                src = at < cn ? psrc[i] + (int64_t)at * a.ldw : zero_chunk;
+            }
+            lds_dma16(src, dst + i * NT * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            const int at = c + qc[i];
+            const uint16_t* src;
+            if (QC) src = at < qlim[i] ? qsrc[i] + at : zero_chunk;
+            else src = at < cn ? qsrc[i] + (int64_t)at * a.lddz : zero_chunk;
+            lds_dma16(src, dst + (PS + i * NT) * 16);
+        }
+    };
+
+    f32x4 acc[FP][FQ];
+    float sum[FQ];
+#pragma unroll
+    for (int i = 0; i < FP; i++)
+#pragma unroll
+        for (int j = 0; j < FQ; j++) acc[i][j] = (f32x4)0.0f;
+#pragma unroll
+    for (int j = 0; j < FQ; j++) sum[j] = 0.0f;
+    const bool sums = DIR == DW && a.db && p0 == 0 && wp == 0;
+
+    s16x8 pf[FP], qf[FQ];
+    auto read = [&](int h, int b) __attribute__((always_inline)) {
+        const lds8_t* pt = (const lds8_t*)lds + b * STAGE;
+        const lds8_t* qt = pt + PS * 16;
+#pragma unroll
+        for (int i = 0; i < FP; i++) pf[i] = PT::frag(pt, wp * (BP / WP) + 16 * i, h, lane);
+#pragma unroll
+        for (int j = 0; j < FQ; j++) qf[j] = QT::frag(qt, wq * (BQ / WQ) + 16 * j, h, lane);
+    };
+    auto multiply = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FP; i++)
+#pragma unroll
+            for (int j = 0; j < FQ; j++) acc[i][j] = mfma<BF>(pf[i], qf[j], acc[i][j]);
+        if (sums)
+#pragma unroll
+            for (int j = 0; j < FQ; j++) sum[j] = add8<BF>(qf[j], sum[j]);
+    };
+
+    if (c0 < cn) {
+        tokens(c0);
+        fill(c0, 0);
+        if (c0 + BK < cn) {
+            tokens(c0 + BK);
+            fill(c0 + BK, 1);
+            tokens(c0 + 2 * BK);
+        }
+        WM_WAIT_VMCNT(0);
+        __syncthreads();
+        int b = 0;
+        for (int c = c0; c < cn; c += BK, b ^= 1) {
+            read(0, b);
+            multiply();
+            read(1, b);
+            multiply();
+            WM_WAIT_VMCNT(0);                   // this wave's part of the next stage
+            __syncthreads();                    // and its last reads of this one
+            if (c + 2 * BK < cn) {
+                fill(c + 2 * BK, b);
+                tokens(c + 3 * BK);
+            }
+        }
+    }
+    if (sums) store_db<FQ>(a, e, q0 + wq * (BQ / WQ), lane, sum);
+    if (DIR == DW && !a.dw) return;
+    store_tile<BF, DIR, FP, FQ, PH>(a, e, p0 + (gated ? wp * (BP / WP / 2) : wp * (BP / WP)), q0 + wq * (BQ / WQ), qn, outs, lane, acc,
+                                    (lf32_t*)lds + wave * epilogue_floats<FP, FQ, PH>());
 }
 
 // ------------------------------------------------------------------ launch
@@ -368,21 +587,37 @@ static int64_t row_tiles(int64_t rows, int64_t E, int bq, bool grouped) {
     return std::min(rows, rows / bq + E);
 }
 
-template <int DIR, int BP, int BQ, int WP, int WQ> static int run(const ProductArgs& a, int64_t qtiles, hipStream_t s) {
+template <int DIR, int BP, int BQ, int WP, int WQ, bool DMA> static int run(const ProductArgs& a, int64_t qtiles, hipStream_t s) {
     const bool gated = DIR == FWD && a.act == WM_ACT_SWIGLU;
     const int outs = DIR == FWD ? (gated ? a.out / 2 : a.out) : a.in, cols = gated ? BP / 2 : BP;
     const int64_t blocks = qtiles * ((outs + cols - 1) / cols);
     if (blocks == 0) return 0;
     if (blocks > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
-    if (a.bf16) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_product<true, DIR, BP, BQ, WP, WQ>), dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
-    else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_product<false, DIR, BP, BQ, WP, WQ>), dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
+    void (*k)(const ProductArgs);
+    if constexpr (DMA) k = a.bf16 ? k_product_dma<true, DIR, BP, BQ, WP, WQ> : k_product_dma<false, DIR, BP, BQ, WP, WQ>;
+    else k = a.bf16 ? k_product<true, DIR, BP, BQ, WP, WQ> : k_product<false, DIR, BP, BQ, WP, WQ>;
+    hipLaunchKernelGGL(k, dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
     return (int)hipGetLastError();
+}
+
+// Whether every 16-byte chunk of the operands is aligned and whole.
+static bool rows16(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+template <int DIR> static bool whole_chunks(const ProductArgs& a) {
+    if (a.in % 8 || (DIR != FWD && (a.out % 8 || !rows16(a.dz, a.lddz)))) return false;
+    if (DIR != DX && !rows16(a.x, a.ldx)) return false;
+    return DIR == DW || (rows16(a.w, a.ldw) && a.w_stride % 8 == 0);
 }
 
 template <int DIR> static int run_rows(const ProductArgs& a, hipStream_t s) {
     const bool grouped = a.offsets != nullptr;
-    if (a.rows / std::max(a.E, 1) <= 32) return run<DIR, 128, 32, 4, 1>(a, row_tiles(a.rows, a.E, 32, grouped), s);
-    return run<DIR, 128, 128, 2, 2>(a, row_tiles(a.rows, a.E, 128, grouped), s);
+    const int64_t per = a.rows / std::max(a.E, 1);
+    if (!whole_chunks<DIR>(a)) {
+        if (per <= 32) return run<DIR, 128, 32, 4, 1, false>(a, row_tiles(a.rows, a.E, 32, grouped), s);
+        return run<DIR, 128, 128, 2, 2, false>(a, row_tiles(a.rows, a.E, 128, grouped), s);
+    }
+    if (per <= 32) return run<DIR, 128, 32, 4, 1, true>(a, row_tiles(a.rows, a.E, 32, grouped), s);
+    if (per <= 128) return run<DIR, 128, 128, 2, 2, true>(a, row_tiles(a.rows, a.E, 128, grouped), s);
+    return run<DIR, 256, 256, 2, 4, true>(a, row_tiles(a.rows, a.E, 256, grouped), s);
 }
 
 int launch_product(const ProductArgs& a, hipStream_t s) { return run_rows<FWD>(a, s); }
@@ -390,7 +625,8 @@ int launch_product_dx(const ProductArgs& a, hipStream_t s) { return run_rows<DX>
 int launch_product_dw(const ProductArgs& args, hipStream_t s) {
     ProductArgs a = args;
     if (!a.dw) a.in = 1;        // db alone: one tile of p
-    return run<DW, 128, 128, 2, 2>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
+    if (!whole_chunks<DW>(a)) return run<DW, 128, 128, 2, 2, false>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
+    return run<DW, 256, 256, 2, 4, true>(a, (int64_t)a.E * ((a.out + 255) / 256), s);
 }
 
 }  // namespace wm
