@@ -111,9 +111,9 @@ SIGNATURES = {
     "wm_expert_ffn": (C.c_int, [_vp, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp, _i64,
                                 _vp]),
     "wm_expert_workspace_size": (_i64, [C.c_int, C.c_int]),
-    "wm_product_workspace_size": (_i64, [C.POINTER(ProductDesc), C.c_int]),
-    "wm_product": (C.c_int, [C.POINTER(ProductDesc), _vp, _i64, _vp]),
-    "wm_product_backward": (C.c_int, [C.POINTER(ProductDesc), _vp, _i64, _vp, _i64, _vp, C.c_int, _vp, _vp, _i64,
+    "wm_product_workspace_size": (_i64, [_vp, C.c_int]),
+    "wm_product": (C.c_int, [_vp, _vp, _i64, _vp]),
+    "wm_product_backward": (C.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, C.c_int, _vp, _vp, _i64,
                                       _vp]),
     "wm_act_backward": (C.c_int, [C.c_int, C.c_int, _i64, C.c_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "wm_group_by_expert": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp]),

@@ -20,60 +20,67 @@ live on the current HIP device.  Every output is rounded once from fp32.
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from ._lib import ACTS, ProductDesc, check, load
-from .moe import _p, _stream
+from ._lib import ACTS, check, load
 
 _TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
+# wm_product_desc as a byte string: filling a ctypes structure field by field
+# takes 3 us of a call whose kernel may take 5.
+_DESC = struct.Struct("8i14q")
+
+
+# Checks cost the host a few microseconds a call, so they are plain Python on
+# what a tensor hands out at once.
 
 def _dev(t: torch.Tensor, name: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA (HIP) tensor")
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch.cuda.current_device():
         raise ValueError(f"{name} is on {t.device}, not on the current device cuda:{torch.cuda.current_device()}")
     return t
 
 
-def _rows(t: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
-    """A matrix of the given shape and type whose rows are contiguous and do not overlap."""
+def _rows(t: torch.Tensor, rows: int, cols: int, dtype, name: str) -> int:
+    """Distance of two rows of a [rows][cols] matrix whose rows are contiguous and do not overlap."""
     _dev(t, name)
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 2 or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if (shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1]):
-        raise ValueError(f"{name} must have contiguous rows, got strides {t.stride()}")
-    return t
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
+        raise ValueError(f"{name} must be {[rows, cols]}, got {list(shape)}")
+    if (cols > 1 and strides[1] != 1) or (rows > 1 and strides[0] < cols):
+        raise ValueError(f"{name} must have contiguous rows, got strides {strides}")
+    return strides[0] if rows > 1 else max(cols, 1)         # a single row's stride means nothing
 
 
-def _dense(t: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
+def _dense(t: torch.Tensor, shape, dtype, name: str) -> int:
+    """Address of a contiguous tensor."""
     _dev(t, name)
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return t
+    return t.data_ptr()
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Distance of two rows in elements (a single row's stride means nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-
-
-def _new(shape, dtype, device, stream) -> torch.Tensor:
+def _new(like: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
     """An output or workspace for work on `stream` (None: the current stream)."""
-    t = torch.empty(shape, dtype=dtype, device=device)
-    if stream is not None and stream != torch.cuda.current_stream():
+    t = like.new_empty(shape, dtype=dtype)
+    if stream is not None:
         t.record_stream(stream)
     return t
+
+
+def _raw(stream, t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device()) if stream is None else stream.cuda_stream
 
 
 def _dtype16(t: torch.Tensor, name: str):
@@ -91,87 +98,109 @@ def _act(act: str) -> int:
 
 def _out_type(dtype, like, name: str):
     dtype = like if dtype is None else dtype
-    if dtype not in (like, torch.float32):
+    if dtype is not like and dtype is not torch.float32:
         raise ValueError(f"{name} must be {like} or float32, got {dtype}")
     return dtype
 
 
-def _desc(x, w, offsets, token) -> ProductDesc:
-    """The operands of a product: w [E][out][in], or [out][in] when offsets is None."""
+def _operands(x, w, offsets, token):
+    """(rows, in, out, E, x rows, offsets, token, x, ldx, w, ldw, w stride) of a product:
+    w [E][out][in], or [out][in] when offsets is None."""
     dt = _dtype16(x, "x")
-    grouped = offsets is not None
-    if w.dim() != (3 if grouped else 2):
-        raise ValueError("w must be [E][out][in]" if grouped else "W must be [out][in]")
-    E, out, inn = w.shape if grouped else (1, *w.shape)
+    _dev(w, "w")
+    shape, strides = w.shape, w.stride()
+    if offsets is None:
+        if len(shape) != 2:
+            raise ValueError("W must be [out][in]")
+        E, (out, inn) = 1, shape
+        off = 0
+    else:
+        if len(shape) != 3:
+            raise ValueError("w must be [E][out][in]")
+        E, out, inn = shape
+        strides = strides[1:]
+        off = _dense(offsets, (E + 1,), torch.int32, "offsets")
     if min(E, out, inn) < 1:
-        raise ValueError(f"the weights are empty: {list(w.shape)}")
+        raise ValueError(f"the weights are empty: {list(shape)}")
+    if w.dtype is not dt:
+        raise ValueError(f"w must be {dt}, got {w.dtype}")
+    if (inn > 1 and strides[1] != 1) or (out > 1 and strides[0] < inn):
+        raise ValueError(f"w must have contiguous rows, got strides {w.stride()}")
+    ldw = strides[0] if out > 1 else inn
+    stride = w.stride(0) if E > 1 else 0
+    if E > 1 and stride < (out - 1) * ldw + inn:
+        raise ValueError(f"the experts of w overlap: strides {w.stride()}")
     if x.dim() != 2:
         raise ValueError(f"x must be [rows][{inn}], got {list(x.shape)}")
-    _rows(x, (x.shape[0], inn), dt, "x")
-    _dev(w, "w")
-    m = w[0] if grouped else w
-    _rows(m, (out, inn), dt, "w")
-    d = ProductDesc()
-    d.dtype, d.inn, d.out, d.n_groups, d.x_rows = _TYPES[dt], inn, out, E, x.shape[0]
-    d.x, d.ldx, d.w, d.ldw = _p(x), _ld(x), _p(w), _ld(m)
-    d.w_stride = w.stride(0) if grouped and E > 1 else out * d.ldw
-    if grouped:
-        d.offsets = _p(_dense(offsets, (E + 1,), torch.int32, "offsets"))
+    x_rows = x.shape[0]
+    ldx = _rows(x, x_rows, inn, dt, "x")
+    rows, tok = x_rows, 0
     if token is not None:
-        d.token = _p(_dense(token, (token.numel(),), torch.int32, "token"))
-    d.rows = x.shape[0] if token is None else token.numel()
-    return d
+        rows = token.numel()
+        tok = _dense(token, (rows,), torch.int32, "token")
+    return rows, inn, out, E, x_rows, off, tok, x.data_ptr(), ldx, w.data_ptr(), ldw, stride
+
+
+def _workspace(L, desc, backward, like, stream):
+    nb = L.wm_product_workspace_size(desc, backward)
+    if nb < 0:
+        check(_lib.WM_EINVAL, "wm_product_workspace_size")
+    return _new(like, (nb,), torch.uint8, stream) if nb else None, nb
 
 
 def _product(x, w, offsets, token, bias, act, residual, out, pre, out_dtype, stream):
-    d = _desc(x, w, offsets, token)
-    d.act = _act(act)
-    if act == "swiglu" and d.out % 2:
-        raise ValueError("SwiGLU needs the gate rows and as many up rows in w")
-    cols = d.out // 2 if act == "swiglu" else d.out
+    rows, inn, outs, E, x_rows, off, tok, xp, ldx, wp, ldw, stride = _operands(x, w, offsets, token)
+    dt, a = x.dtype, _act(act)
+    cols = outs
+    if act == "swiglu":
+        if outs % 2:
+            raise ValueError("SwiGLU needs the gate rows and as many up rows in w")
+        cols = outs // 2
+    bp = rp = ldr = pp = ldp = 0
     if bias is not None:
-        d.bias = _p(_dense(bias, w.shape[:-1], x.dtype, "bias"))
+        bp = _dense(bias, w.shape[:-1], dt, "bias")
     if residual is not None:
-        d.residual, d.ld_residual = _p(_rows(residual, (d.rows, cols), x.dtype, "residual")), _ld(residual)
-    if out is not None and out_dtype is None:
-        out_dtype = out.dtype
-    yt = _out_type(out_dtype, x.dtype, "out_dtype")
-    y = _new((d.rows, cols), yt, x.device, stream) if out is None else _rows(out, (d.rows, cols), yt, "out")
-    d.y, d.ldy, d.y_type = _p(y), _ld(y), _TYPES[yt]
+        rp, ldr = residual.data_ptr(), _rows(residual, rows, cols, dt, "residual")
+    if out is None:
+        yt = _out_type(out_dtype, dt, "out_dtype")
+        out, ldy = _new(x, (rows, cols), yt, stream), cols
+    else:
+        yt = _out_type(out.dtype if out_dtype is None else out_dtype, dt, "out_dtype")
+        ldy = _rows(out, rows, cols, yt, "out")
     if pre is not None:
-        d.pre, d.ld_pre = _p(_rows(pre, (d.rows, d.out), x.dtype, "pre")), _ld(pre)
+        pp, ldp = pre.data_ptr(), _rows(pre, rows, outs, dt, "pre")
+    desc = _DESC.pack(_TYPES[dt], rows, inn, outs, E, x_rows, a, _TYPES[yt], off, tok, xp, ldx, wp, ldw, stride, bp,
+                      rp, ldr, out.data_ptr(), ldy, pp, ldp)
     L = load()
-    ws, nb = _workspace(L, d, 0, x.device, stream)
-    check(L.wm_product(C.byref(d), _p(ws), nb, _stream(stream)), "wm_product")
-    return y
-
-
-def _workspace(L, d, backward, device, stream):
-    nb = L.wm_product_workspace_size(C.byref(d), backward)
-    if nb < 0:
-        check(_lib.WM_EINVAL, "wm_product_workspace_size")
-    return (_new((nb,), torch.uint8, device, stream), nb) if nb else (None, 0)
+    ws, nb = _workspace(L, desc, 0, x, stream)
+    check(L.wm_product(desc, ws.data_ptr() if nb else None, nb, _raw(stream, x)), "wm_product")
+    return out
 
 
 def _product_backward(dz, x, w, offsets, token, need_dx, need_dw, need_db, dw_dtype, dx, dw, db, stream):
-    d = _desc(x, w, offsets, token)
-    _rows(dz, (d.rows, d.out), x.dtype, "dz")
-    if dw is not None and dw_dtype is None:
-        dw_dtype = dw.dtype
-    wt = _out_type(dw_dtype, x.dtype, "dw_dtype")
+    rows, inn, outs, E, x_rows, off, tok, xp, ldx, wp, ldw, stride = _operands(x, w, offsets, token)
+    dt = x.dtype
+    ldz = _rows(dz, rows, outs, dt, "dz")
+    wt = _out_type(dw.dtype if dw is not None and dw_dtype is None else dw_dtype, dt, "dw_dtype")
+    dxp = lddx = dwp = dbp = 0
     if need_dx or dx is not None:
-        shape = (d.rows, d.inn)
-        dx = _new(shape, x.dtype, x.device, stream) if dx is None else _rows(dx, shape, x.dtype, "dx")
+        if dx is None:
+            dx = _new(x, (rows, inn), dt, stream)
+        dxp, lddx = dx.data_ptr(), _rows(dx, rows, inn, dt, "dx")
     if need_dw or dw is not None:
-        dw = _new(w.shape, wt, x.device, stream) if dw is None else _dense(dw, w.shape, wt, "dw")
+        if dw is None:
+            dw = _new(x, w.shape, wt, stream)
+        dwp = _dense(dw, w.shape, wt, "dw")
     if need_db or db is not None:
-        shape = w.shape[:-1]
-        db = (_new(shape, torch.float32, x.device, stream) if db is None
-              else _dense(db, shape, torch.float32, "db"))
+        if db is None:
+            db = _new(x, w.shape[:-1], torch.float32, stream)
+        dbp = _dense(db, w.shape[:-1], torch.float32, "db")
+    desc = _DESC.pack(_TYPES[dt], rows, inn, outs, E, x_rows, 0, _TYPES[dt], off, tok, xp, ldx, wp, ldw, stride,
+                      0, 0, 0, 0, 0, 0, 0)
     L = load()
-    ws, nb = _workspace(L, d, 1, x.device, stream)
-    check(L.wm_product_backward(C.byref(d), _p(dz), _ld(dz), _p(dx), _ld(dx) if dx is not None else 0, _p(dw),
-                                _TYPES[wt], _p(db), _p(ws), nb, _stream(stream)), "wm_product_backward")
+    ws, nb = _workspace(L, desc, 1, x, stream)
+    check(L.wm_product_backward(desc, dz.data_ptr(), ldz, dxp, lddx, dwp, _TYPES[wt], dbp,
+                                ws.data_ptr() if nb else None, nb, _raw(stream, x)), "wm_product_backward")
     return dx, dw, db
 
 
@@ -209,13 +238,12 @@ def group_by_expert(ids: torch.Tensor, E: int, stream=None) -> Grouping:
     _dev(ids, "ids")
     if ids.dim() != 2 or ids.shape[1] < 1:
         raise ValueError(f"ids must be [T][K], got {list(ids.shape)}")
-    _dense(ids, ids.shape, torch.int32, "ids")
+    p = _dense(ids, ids.shape, torch.int32, "ids")
     if E < 1:
         raise ValueError("there must be an expert")
     T, K = ids.shape
-    g = Grouping(*(_new(s, torch.int32, ids.device, stream) for s in ((E + 1,), (T * K,), (T, K))))
-    check(load().wm_group_by_expert(_p(ids), T, K, E, _p(g.offsets), _p(g.token), _p(g.row), _stream(stream)),
-          "wm_group_by_expert")
+    g = Grouping(*(_new(ids, s, torch.int32, stream) for s in ((E + 1,), (T * K,), (T, K))))
+    check(load().wm_group_by_expert(p, T, K, E, *(t.data_ptr() for t in g), _raw(stream, ids)), "wm_group_by_expert")
     return g
 
 
@@ -246,31 +274,31 @@ def grouped_matmul_backward(dz: torch.Tensor, x: torch.Tensor, w: torch.Tensor, 
 def act_backward(dy: torch.Tensor, pre: torch.Tensor, act: str, out: Optional[torch.Tensor] = None,
                  stream=None) -> torch.Tensor:
     """dz = act'(pre) * dy.  dy [T][n]; pre and the result [T][n], or [T][2 n] for "swiglu".  out may be pre."""
-    dt = _dtype16(pre, "pre")
+    dt, a = _dtype16(pre, "pre"), _act(act)
     if dy.dim() != 2 or dy.shape[1] < 1:
         raise ValueError(f"dy must be [rows][columns], got {list(dy.shape)}")
     T, n = dy.shape
-    wide = (T, 2 * n if _act(act) == ACTS["swiglu"] else n)
-    _rows(dy, (T, n), dt, "dy")
-    _rows(pre, wide, dt, "pre")
-    dz = _new(wide, dt, pre.device, stream) if out is None else _rows(out, wide, dt, "out")
-    check(load().wm_act_backward(_TYPES[dt], ACTS[act], T, n, _p(dy), _ld(dy), _p(pre), _ld(pre), _p(dz), _ld(dz),
-                                 _stream(stream)), "wm_act_backward")
+    wide = 2 * n if act == "swiglu" else n
+    ldy, ldp = _rows(dy, T, n, dt, "dy"), _rows(pre, T, wide, dt, "pre")
+    dz = _new(pre, (T, wide), dt, stream) if out is None else out
+    ldz = _rows(dz, T, wide, dt, "out")
+    check(load().wm_act_backward(_TYPES[dt], a, T, n, dy.data_ptr(), ldy, pre.data_ptr(), ldp, dz.data_ptr(), ldz,
+                                 _raw(stream, pre)), "wm_act_backward")
     return dz
 
 
 def _combine_args(y, row, w):
+    """(type, T, K, H, distance of y's rows, row, w)."""
     dt = _dtype16(y, "y")
     if y.dim() != 2 or y.shape[1] < 1:
         raise ValueError(f"y must be [rows][H], got {list(y.shape)}")
-    _rows(y, y.shape, dt, "y")
+    ldy = _rows(y, *y.shape, dt, "y")
     _dev(row, "row")
     if row.dim() != 2:
         raise ValueError(f"row must be [T][K], got {list(row.shape)}")
-    _dense(row, row.shape, torch.int32, "row")
-    if w is not None:
-        _dense(w, row.shape, torch.float32, "w")
-    return dt, row.shape[0], row.shape[1], y.shape[1]
+    rp = _dense(row, row.shape, torch.int32, "row")
+    wp = 0 if w is None else _dense(w, row.shape, torch.float32, "w")
+    return dt, row.shape[0], row.shape[1], y.shape[1], ldy, rp, wp
 
 
 def combine(y: torch.Tensor, row: torch.Tensor, w: Optional[torch.Tensor] = None,
@@ -281,18 +309,17 @@ def combine(y: torch.Tensor, row: torch.Tensor, w: Optional[torch.Tensor] = None
     y [rows][H] 16-bit, row int32 [T][K], w float32 [T][K] (None: ones),
     residual [T][H] of the result's type: y's or float32.  A row outside y
     (-1: padding) adds nothing, whatever its weight.  residual may be out."""
-    dt, T, K, H = _combine_args(y, row, w)
-    if out is not None and out_dtype is None:
-        out_dtype = out.dtype
-    if out is None and out_dtype is None and residual is not None:
-        out_dtype = residual.dtype
+    dt, T, K, H, ldy, rp, wp = _combine_args(y, row, w)
+    if out_dtype is None and (out is not None or residual is not None):
+        out_dtype = (residual if out is None else out).dtype
     ot = _out_type(out_dtype, dt, "out_dtype")
-    o = _new((T, H), ot, y.device, stream) if out is None else _rows(out, (T, H), ot, "out")
+    o = _new(y, (T, H), ot, stream) if out is None else out
+    ldo = _rows(o, T, H, ot, "out")
+    sp = ldr = 0
     if residual is not None:
-        _rows(residual, (T, H), ot, "residual")
-    check(load().wm_combine_rows(_TYPES[dt], _p(y), _ld(y), y.shape[0], _p(row), _p(w), T, K, H, _p(residual),
-                                 _ld(residual) if residual is not None else 0, _p(o), _ld(o), _TYPES[ot],
-                                 _stream(stream)), "wm_combine_rows")
+        sp, ldr = residual.data_ptr(), _rows(residual, T, H, ot, "residual")
+    check(load().wm_combine_rows(_TYPES[dt], y.data_ptr(), ldy, y.shape[0], rp, wp, T, K, H, sp, ldr, o.data_ptr(), ldo,
+                                 _TYPES[ot], _raw(stream, y)), "wm_combine_rows")
     return o
 
 
@@ -303,13 +330,19 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, row: torch.Tensor, w: 
     Every row of y may be named by one pick only.  Rows that none names are
     left as they are in dy (unspecified in a new one); dw is 0 where the row
     is outside y.  The residual's gradient is dout itself."""
-    dt, T, K, H = _combine_args(y, row, w)
+    dt, T, K, H, ldy, rp, wp = _combine_args(y, row, w)
     gt = _out_type(dout.dtype, dt, "dout's type")
-    _rows(dout, (T, H), gt, "dout")
+    ldg = _rows(dout, T, H, gt, "dout")
+    dyp = lddy = dwp = 0
+    dw = None
     if need_dy or dy is not None:
-        dy = _new(y.shape, dt, y.device, stream) if dy is None else _rows(dy, y.shape, dt, "dy")
-    dw = _new((T, K), torch.float32, y.device, stream) if need_dw else None
-    check(load().wm_combine_rows_backward(_TYPES[dt], _p(dout), _ld(dout), _TYPES[gt], _p(y), _ld(y), y.shape[0],
-                                          _p(row), _p(w), T, K, H, _p(dy), _ld(dy) if dy is not None else 0, _p(dw),
-                                          _stream(stream)), "wm_combine_rows_backward")
+        if dy is None:
+            dy = _new(y, y.shape, dt, stream)
+        dyp, lddy = dy.data_ptr(), _rows(dy, *y.shape, dt, "dy")
+    if need_dw:
+        dw = _new(y, (T, K), torch.float32, stream)
+        dwp = dw.data_ptr()
+    check(load().wm_combine_rows_backward(_TYPES[dt], dout.data_ptr(), ldg, _TYPES[gt], y.data_ptr(), ldy, y.shape[0],
+                                          rp, wp, T, K, H, dyp, lddy, dwp, _raw(stream, y)),
+          "wm_combine_rows_backward")
     return dy, dw
