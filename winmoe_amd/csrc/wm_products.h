@@ -43,6 +43,10 @@ struct ProductArgs {
     void* dw;                   // [E][out][in], dense
     int dw_f32;
     float* db;                  // [E][out]
+    // parts of the contraction: each leaves fp32 sums [split][row][column] (and
+    // [split][E * out] of db), which a second kernel adds in order
+    int split;                  // 1: none
+    float *part, *part_db;
 };
 
 int launch_product(const ProductArgs& a, hipStream_t s);

@@ -18,6 +18,8 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
+#include <stdlib.h>
 
 #include "../../include/winmoe_hip.h"
 #include "wm_act.h"
@@ -60,37 +62,62 @@ WM_DEV uint4 load8(const uint16_t* p, int n) {
 struct GroupTile {
     int e, start, n, tile;      // e < 0: past the last tile
 };
+WM_DEV int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);     // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);     // lane 15 of a row into the next, then of both
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+// 512 groups at a time, 8 per lane, all loads in flight together.
 WM_DEV GroupTile find_tile(const int32_t* __restrict__ offsets, int E, int rows, int bq, int qt) {
     GroupTile g{-1, 0, 0, 0};
     if (!offsets) {
-        g.e = qt * bq < rows ? 0 : -1;
+        g.e = (int64_t)qt * bq < rows ? 0 : -1;
         g.n = rows;
         g.tile = qt;
         return g;
     }
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, shift = __builtin_ctz(bq);      // bq is a power of two
     int before = 0;
-    for (int e0 = 0; e0 < E; e0 += 64) {
-        const int e = e0 + lane;
-        const int a = e < E ? min(max(offsets[e], 0), rows) : 0;
-        const int b = e < E ? min(max(offsets[e + 1], a), rows) : 0;
-        const int t = (b - a + bq - 1) / bq;
-        int sum = t;
+    for (int e0 = 0; e0 < E; e0 += 512) {
+        const int base = e0 + 8 * lane;
+        int off[9], sum = 0;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(sum, d);
-            if (lane >= d) sum += v;
+        for (int i = 0; i < 9; i++) off[i] = offsets[min(base + i, E)];
+        off[0] = min(max(off[0], 0), rows);
+#pragma unroll
+        for (int i = 1; i < 9; i++) {
+            const int v = min(max(off[i], 0), rows);
+            off[i] = v;
+            sum += (max(v - off[i - 1], 0) + bq - 1) >> shift;
         }
-        const uint64_t hit = __ballot(before + sum > qt);
+        const int end = before + wave_scan(sum);
+        const uint64_t hit = __ballot(end > qt);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            g.e = e0 + l;
-            g.start = __builtin_amdgcn_readlane(a, l);
-            g.n = __builtin_amdgcn_readlane(b, l) - g.start;
-            g.tile = qt - (before + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(t, l));
+            int at = end - sum, e = base, start = off[0], n = 0;
+            bool found = false;
+#pragma unroll
+            for (int i = 1; i < 9; i++) {
+                const int m = max(off[i] - off[i - 1], 0), t = (m + bq - 1) >> shift;
+                if (!found) {
+                    e = base + i - 1;
+                    start = off[i - 1];
+                    n = m;
+                    found = at + t > qt;
+                    at += found ? 0 : t;
+                }
+            }
+            g.e = __builtin_amdgcn_readlane(e, l);
+            g.start = __builtin_amdgcn_readlane(start, l);
+            g.n = __builtin_amdgcn_readlane(n, l);
+            g.tile = qt - __builtin_amdgcn_readlane(at, l);
             return g;
         }
-        before += __builtin_amdgcn_readlane(sum, 63);
+        before = __builtin_amdgcn_readlane(end, 63);
     }
     return g;
 }
@@ -110,24 +137,27 @@ WM_DEV TileId tile_id(int block, int blocks, int nP) {
 
 // ------------------------------------------------------------------ LDS tiles
 
-// [TILE][64], memory rows along the contraction.  Slot s (16 bytes) holds
-// chunk (s & 7) ^ (index & 7) of row index = s >> 3.
-template <int TILE> struct AlongC {
+// [TILE][KB], memory rows along the contraction.  A row's 16-byte chunks are
+// permuted by its index, so that the 16 rows of a read fall on all banks.
+template <int TILE, int KB> struct AlongC {
+    static constexpr int CH = KB / 8;
+    WM_DEV static int perm(int index) { return KB == 64 ? index & 7 : (index >> 1) & 3; }
+    // what slot s (16 bytes) holds
     WM_DEV static void slot(int s, int& index, int& c) {
-        index = s >> 3;
-        c = 8 * ((s & 7) ^ (index & 7));
+        index = s / CH;
+        c = 8 * ((s % CH) ^ perm(index));
     }
     // operand of 16 indices from `base` on, 32 contraction steps from 32 * ks on
     WM_DEV static s16x8 frag(const lds8_t* t, int base, int ks, int lane) {
-        const int i = base + (lane & 15), ch = (4 * ks + (lane >> 4)) ^ (lane & 7);
-        return *(const __attribute__((address_space(3))) s16x8*)(t + 128 * i + 16 * ch);
+        const int i = base + (lane & 15), ch = (4 * ks + (lane >> 4)) ^ perm(lane & 15);
+        return *(const __attribute__((address_space(3))) s16x8*)(t + 2 * KB * i + 16 * ch);
     }
 };
 
-// [64][TILE], memory rows are contraction steps.  Units of 16 values are
+// [KB][TILE], memory rows are contraction steps.  Units of 16 values are
 // permuted within a row by the row's bits 0, 1 and 3, which the 16 rows of a
 // transposing read run through.
-template <int TILE> struct AcrossC {
+template <int TILE, int KB> struct AcrossC {
     static constexpr int CH = TILE / 8, U = TILE / 16;
     WM_DEV static int perm(int c) { return ((c & 3) | ((c >> 1) & 4)) & (U - 1); }
     WM_DEV static void slot(int s, int& index, int& c) {
@@ -147,6 +177,47 @@ template <int TILE> struct AcrossC {
 
 // ------------------------------------------------------------------ epilogue
 
+// 8 outputs of row q from column p on, from their sums (up: SwiGLU's up half).
+template <bool BF, int DIR> WM_DEV void store8(const ProductArgs& a, int e, int q, int p, int outs, float (&z)[8], float (&up)[8]) {
+    const int n = outs - p;
+    if constexpr (DIR == FWD) {
+        const bool gated = a.act == WM_ACT_SWIGLU;
+        float v[8];
+        if (a.bias) {
+            const uint16_t* b = a.bias + (int64_t)e * a.out + p;
+            get8<BF>(b, n, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) z[i] += v[i];
+            if (gated) {
+                get8<BF>(b + outs, n, v);
+#pragma unroll
+                for (int i = 0; i < 8; i++) up[i] += v[i];
+            }
+        }
+        if (a.pre) {
+            uint16_t* pre = a.pre + (int64_t)q * a.ldpre + p;
+            put8<BF>(pre, n, z);
+            if (gated) put8<BF>(pre + outs, n, up);
+        }
+        if (a.act != WM_ACT_NONE)
+#pragma unroll
+            for (int i = 0; i < 8; i++) z[i] = act_value(a.act, z[i], up[i]);
+        if (a.res) {
+            get8<BF>(a.res + (int64_t)q * a.ldres + p, n, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) z[i] += v[i];
+        }
+        if (a.y_f32) putf8((float*)a.y + (int64_t)q * a.ldy + p, n, z);
+        else put8<BF>((uint16_t*)a.y + (int64_t)q * a.ldy + p, n, z);
+    } else if constexpr (DIR == DX) {
+        put8<BF>(a.dx + (int64_t)q * a.lddx + p, n, z);
+    } else {
+        const int64_t at = ((int64_t)e * a.out + q) * a.in + p;
+        if (a.dw_f32) putf8((float*)a.dw + at, n, z);
+        else put8<BF>((uint16_t*)a.dw + at, n, z);
+    }
+}
+
 // A wave's FP x FQ fragments go through LDS, PH parts one after another, so
 // that a lane then holds 8 consecutive outputs of one row: one 16-byte store
 // (and bias or residual load) per row and lane instead of two of 8 bytes that
@@ -157,7 +228,7 @@ template <int FP, int FQ, int PH> constexpr int epilogue_floats() { return FQ / 
 
 // Outputs from p0 on (contiguous) of rows from q0 on, below qn.  lds: the wave's own.
 template <bool BF, int DIR, int FP, int FQ, int PH>
-WM_DEV void store_tile(const ProductArgs& a, int e, int p0, int q0, int qn, int outs, int lane, const f32x4 (&acc)[FP][FQ],
+WM_DEV void store_tile(const ProductArgs& a, int e, int part, int p0, int q0, int qn, int outs, int lane, const f32x4 (&acc)[FP][FQ],
                        lf32_t* lds) {
     constexpr int ROW = FP * 16 + 4;
     typedef __attribute__((address_space(3))) f32x4 lf32x4;
@@ -181,46 +252,38 @@ WM_DEV void store_tile(const ProductArgs& a, int e, int p0, int q0, int qn, int 
             float z[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) z[i] = src[i];
-            if constexpr (DIR == FWD) {
-                float up[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8];
-                if (gated)
+            float up[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) up[i] = src[16 + i];
-                if (a.bias) {
-                    const uint16_t* b = a.bias + (int64_t)e * a.out + p;
-                    get8<BF>(b, n, v);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) z[i] += v[i];
-                    if (gated) {
-                        get8<BF>(b + outs, n, v);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) up[i] += v[i];
-                    }
-                }
-                if (a.pre) {
-                    uint16_t* pre = a.pre + (int64_t)q * a.ldpre + p;
-                    put8<BF>(pre, n, z);
-                    if (gated) put8<BF>(pre + outs, n, up);
-                }
-                if (a.act != WM_ACT_NONE)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) z[i] = act_value(a.act, z[i], up[i]);
-                if (a.res) {
-                    get8<BF>(a.res + (int64_t)q * a.ldres + p, n, v);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) z[i] += v[i];
-                }
-                if (a.y_f32) putf8((float*)a.y + (int64_t)q * a.ldy + p, n, z);
-                else put8<BF>((uint16_t*)a.y + (int64_t)q * a.ldy + p, n, z);
-            } else if constexpr (DIR == DX) {
-                put8<BF>(a.dx + (int64_t)q * a.lddx + p, n, z);
+            for (int i = 0; i < 8; i++) up[i] = gated ? src[16 + i] : 0.0f;
+            if (a.split > 1) {
+                const int64_t at = DIR == DW ? (int64_t)(part * a.E + e) * a.out + q : (int64_t)part * a.rows + q;
+                float* d = a.part + at * (DIR == FWD ? a.out : a.in) + p;
+                putf8(d, n, z);
+                if (gated) putf8(d + outs, n, up);
             } else {
-                const int64_t at = ((int64_t)e * a.out + q) * a.in + p;
-                if (a.dw_f32) putf8((float*)a.dw + at, n, z);
-                else put8<BF>((uint16_t*)a.dw + at, n, z);
+                store8<BF, DIR>(a, e, q, p, outs, z, up);
             }
         }
     }
+}
+
+// One output of the forward product, from its sums.
+template <bool BF> WM_DEV void store_one(const ProductArgs& a, int e, int q, int p, int outs, float z, float u) {
+    const bool gated = a.act == WM_ACT_SWIGLU;
+    if (a.bias) {
+        const uint16_t* b = a.bias + (int64_t)e * a.out + p;
+        z += from16<BF>(b[0]);
+        if (gated) u += from16<BF>(b[outs]);
+    }
+    if (a.pre) {
+        uint16_t* pre = a.pre + (int64_t)q * a.ldpre + p;
+        pre[0] = to16<BF>(z);
+        if (gated) pre[outs] = to16<BF>(u);
+    }
+    z = act_value(a.act, z, u);
+    if (a.res) z += from16<BF>(a.res[(int64_t)q * a.ldres + p]);
+    if (a.y_f32) ((float*)a.y)[(int64_t)q * a.ldy + p] = z;
+    else ((uint16_t*)a.y)[(int64_t)q * a.ldy + p] = to16<BF>(z);
 }
 
 // Sum of an operand's 8 values of one column, added to s.
@@ -231,14 +294,14 @@ template <bool BF> WM_DEV float add8(s16x8 v, float s) {
 }
 
 // db of the wave's columns: lane l summed the steps of its quarter for column l % 16.
-template <int FQ> WM_DEV void store_db(const ProductArgs& a, int e, int q0, int lane, const float (&sum)[FQ]) {
+template <int FQ> WM_DEV void store_db(const ProductArgs& a, int e, int part, int q0, int lane, const float (&sum)[FQ]) {
 #pragma unroll
     for (int j = 0; j < FQ; j++) {
         float s = sum[j];
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
         const int q = q0 + 16 * j + lane;
-        if (lane < 16 && q < a.out) a.db[(int64_t)e * a.out + q] = s;
+        if (lane < 16 && q < a.out) (a.split > 1 ? a.part_db + (int64_t)part * a.E * a.out : a.db)[(int64_t)e * a.out + q] = s;
     }
 }
 
@@ -251,8 +314,8 @@ template <bool BF, int DIR, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     constexpr int NT = 64 * WP * WQ, FP = BP / WP / 16, FQ = BQ / WQ / 16;
     constexpr bool PC = DIR == FWD, QC = DIR != DW;         // operand's rows run along the contraction
-    using PT = typename std::conditional<PC, AlongC<BP>, AcrossC<BP>>::type;
-    using QT = typename std::conditional<QC, AlongC<BQ>, AcrossC<BQ>>::type;
+    using PT = typename std::conditional<PC, AlongC<BP, BK>, AcrossC<BP, BK>>::type;
+    using QT = typename std::conditional<QC, AlongC<BQ, BK>, AcrossC<BQ, BK>>::type;
     constexpr int PS = BP * 8, QS = BQ * 8, NP = (PS + NT - 1) / NT, NQ = (QS + NT - 1) / NT;
     constexpr int STAGE = (BP + BQ) * 2 * BK, PH = 1, EPI = WP * WQ * 4 * epilogue_floats<FP, FQ, PH>();
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE > EPI ? 2 * STAGE : EPI];
@@ -385,9 +448,9 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
         __syncthreads();
     }
 
-    if (sums) store_db<FQ>(a, e, q0 + wq * (BQ / WQ), lane, sum);
+    if (sums) store_db<FQ>(a, e, 0, q0 + wq * (BQ / WQ), lane, sum);
     if (DIR == DW && !a.dw) return;
-    store_tile<BF, DIR, FP, FQ, PH>(a, e, p0 + (gated ? wp * (BP / WP / 2) : wp * (BP / WP)), q0 + wq * (BQ / WQ), qn, outs, lane, acc,
+    store_tile<BF, DIR, FP, FQ, PH>(a, e, 0, p0 + (gated ? wp * (BP / WP / 2) : wp * (BP / WP)), q0 + wq * (BQ / WQ), qn, outs, lane, acc,
                                     (lf32_t*)lds + wave * epilogue_floats<FP, FQ, PH>());
 }
 
@@ -403,26 +466,29 @@ WM_DEV void lds_dma16(const void* src, lds8_t* dst) {
 // Read in place of chunks that do not exist.
 static __device__ __attribute__((aligned(16))) uint16_t zero_chunk[8];
 
-// The same tile with LDS-DMA: two stages of 64 contraction steps, filled while
-// the other one is used.  The operands of a half stage (32 steps) are read
-// into registers while the products of the half before run, across the stage
-// boundary too: at the middle of stage k every wave waits for its part of
-// stage k + 1 and its last reads of stage k, and after the barrier fills stage
-// k + 2 into the buffer just left.  One barrier per stage.
+// The same tile with LDS-DMA: a ring of S stages of 64 contraction steps, S - 1
+// of them in flight or in use at any time.  One barrier per stage: behind it
+// every wave's part of the stage has landed and every wave is done with the
+// stage before, whose buffer is filled again at once.
 //
-// Every chunk of 8 values exists whole or not at all (operand_rules()); rows
+// Every chunk of 8 values exists whole or not at all (whole_chunks()); rows
 // and columns past the matrix repeat valid ones, as their results are not
 // stored, and steps past the end of the contraction are zeros in both operands.
-template <bool BF, int DIR, int BP, int BQ, int WP, int WQ>
+//
+// A call with too few tiles to fill the chip gives each tile's contraction to
+// a.split workgroups (k_join adds their sums).
+template <bool BF, int DIR, int BP, int BQ, int WP, int WQ, int S, int BK>
 __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs a) {
     constexpr int NT = 64 * WP * WQ, FP = BP / WP / 16, FQ = BQ / WQ / 16;
     constexpr bool PC = DIR == FWD, QC = DIR != DW;
-    using PT = typename std::conditional<PC, AlongC<BP>, AcrossC<BP>>::type;
-    using QT = typename std::conditional<QC, AlongC<BQ>, AcrossC<BQ>>::type;
-    constexpr int PS = BP * 8, QS = BQ * 8, NP = PS / NT, NQ = QS / NT, STAGE = (BP + BQ) * 2 * BK;
+    using PT = typename std::conditional<PC, AlongC<BP, BK>, AcrossC<BP, BK>>::type;
+    using QT = typename std::conditional<QC, AlongC<BQ, BK>, AcrossC<BQ, BK>>::type;
+    constexpr int PS = BP * BK / 8, QS = BQ * BK / 8, NP = PS / NT, NQ = QS / NT, STAGE = (BP + BQ) * 2 * BK;
     static_assert(PS % NT == 0 && QS % NT == 0, "whole chunks per thread");
+    static_assert((S - 2) * (NP + NQ) < 64, "loads are counted");
     constexpr int PH = WP * WQ * 4 * epilogue_floats<FP, FQ, 1>() > 160 * 1024 ? 2 : 1, EPI = WP * WQ * 4 * epilogue_floats<FP, FQ, PH>();
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE > EPI ? 2 * STAGE : EPI];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[NT == 512 && DIR != DW ? STAGE / 2 * 5 : S * STAGE > EPI ? S * STAGE : EPI];
+    static_assert(sizeof(lds) >= EPI, "the epilogue fits");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wp = wave % WP, wq = wave / WP;
@@ -430,7 +496,8 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
     const int outs = DIR == FWD ? (gated ? a.out / 2 : a.out) : a.in;
     const int cols = gated ? BP / 2 : BP;
     const int nP = (outs + cols - 1) / cols;
-    const TileId id = tile_id(blockIdx.x, gridDim.x, nP);
+    const int tiles = gridDim.x / a.split, part = blockIdx.x / tiles;
+    const TileId id = tile_id(blockIdx.x % tiles, tiles, nP);
     const int p0 = id.p * cols;
     int e, q0, qn, c0 = 0, cn;
     const uint16_t* w = nullptr;
@@ -449,6 +516,12 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
         qn = g.start + g.n;
         cn = DIR == FWD ? a.in : a.out;
         w = a.w + (int64_t)e * a.w_stride;
+    }
+
+    if (a.split > 1) {
+        const int n = (cn - c0 + BK - 1) / BK, first = c0;
+        c0 = first + BK * (int)((int64_t)n * part / a.split);
+        cn = min(cn, first + BK * (int)((int64_t)n * (part + 1) / a.split));
     }
 
     // AlongC: src = the chunk's row at its column, lim = where the row ends.
@@ -487,37 +560,39 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
             qsrc[i] = a.dz + (q0 + ix < qn ? q0 + ix : q0);
         }
     }
-    // DW gathers rows of x: the tokens of a stage are loaded one stage ahead
-    int tok[NP];
-    auto tokens = [&](int c) __attribute__((always_inline)) {
-        if (DIR == DW && a.token)
+    // DW gathers rows of x: a load of 64 chunks covers 64 / (BP / 8) rows, whose
+    // tokens come through scalar loads (vector loads would wait for the stages
+    // in flight before them)
+    auto token = [&](int c, int i) __attribute__((always_inline)) {
+        constexpr int R = 512 / BP;
+        const int r = c + (64 * wave + i * NT) / (BP / 8);
+        int t = -1;
 #pragma unroll
-            for (int i = 0; i < NP; i++) tok[i] = c + pc[i] < cn ? a.token[c + pc[i]] : -1;
+        for (int k = 0; k < R; k++) {
+            const int v = r + k < cn ? ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)a.token)[r + k] : -1;
+            t = R == 1 || lane / (64 / R) == k ? v : t;
+        }
+        return t;
     };
-    auto fill = [&](int c, int b) __attribute__((always_inline)) {
-        lds8_t* dst = (lds8_t*)lds + b * STAGE + 1024 * wave;
-#pragma unroll
-        for (int i = 0; i < NP; i++) {
-            const int at = c + pc[i];
-            const uint16_t* src;
-            if (PC) {
-                src = at < plim[i] ? psrc[i] + at : zero_chunk;
-            } else if (DIR == DW) {
-                const int t = a.token ? tok[i] : at;
-                src = at < cn && (uint32_t)t < (uint32_t)a.x_rows ? psrc[i] + (int64_t)t * a.ldx : zero_chunk;
-            } else {
-                src = at < cn ? psrc[i] + (int64_t)at * a.ldw : zero_chunk;
-            }
-            lds_dma16(src, dst + i * NT * 16);
+    auto fill_p = [&](int c, int i, lds8_t* dst) __attribute__((always_inline)) {
+        const int at = c + pc[i];
+        const uint16_t* src;
+        if (PC) {
+            src = at < plim[i] ? psrc[i] + at : zero_chunk;
+        } else if (DIR == DW) {
+            const int t = a.token ? token(c, i) : at;
+            src = at < cn && (uint32_t)t < (uint32_t)a.x_rows ? psrc[i] + (int64_t)t * a.ldx : zero_chunk;
+        } else {
+            src = at < cn ? psrc[i] + (int64_t)at * a.ldw : zero_chunk;
         }
-#pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            const int at = c + qc[i];
-            const uint16_t* src;
-            if (QC) src = at < qlim[i] ? qsrc[i] + at : zero_chunk;
-            else src = at < cn ? qsrc[i] + (int64_t)at * a.lddz : zero_chunk;
-            lds_dma16(src, dst + (PS + i * NT) * 16);
-        }
+        lds_dma16(src, dst + 1024 * wave + i * NT * 16);
+    };
+    auto fill_q = [&](int c, int i, lds8_t* dst) __attribute__((always_inline)) {
+        const int at = c + qc[i];
+        const uint16_t* src;
+        if (QC) src = at < qlim[i] ? qsrc[i] + at : zero_chunk;
+        else src = at < cn ? qsrc[i] + (int64_t)at * a.lddz : zero_chunk;
+        lds_dma16(src, dst + 1024 * wave + i * NT * 16);
     };
 
     f32x4 acc[FP][FQ];
@@ -531,9 +606,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
     const bool sums = DIR == DW && a.db && p0 == 0 && wp == 0;
 
     s16x8 pf[FP], qf[FQ];
-    auto read = [&](int h, int b) __attribute__((always_inline)) {
-        const lds8_t* pt = (const lds8_t*)lds + b * STAGE;
-        const lds8_t* qt = pt + PS * 16;
+    auto read = [&](int h, const lds8_t* pt, const lds8_t* qt) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < FP; i++) pf[i] = PT::frag(pt, wp * (BP / WP) + 16 * i, h, lane);
 #pragma unroll
@@ -549,34 +622,250 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
             for (int j = 0; j < FQ; j++) sum[j] = add8<BF>(qf[j], sum[j]);
     };
 
-    if (c0 < cn) {
-        tokens(c0);
-        fill(c0, 0);
-        if (c0 + BK < cn) {
-            tokens(c0 + BK);
-            fill(c0 + BK, 1);
-            tokens(c0 + 2 * BK);
-        }
-        WM_WAIT_VMCNT(0);
-        __syncthreads();
-        int b = 0;
-        for (int c = c0; c < cn; c += BK, b ^= 1) {
-            read(0, b);
+    if constexpr (NT == 512 && DIR != DW) {
+        // Two groups of 4 waves, one of each group per SIMD, take turns: while
+        // one reads its operands of half a stage the other one multiplies.  Time
+        // runs in slots that end in a barrier: group 0 reads the halves of stage
+        // k in slots 4 k and 4 k + 2 and multiplies in slots 4 k + 1 and 4 k + 3,
+        // group 1 does so one slot later.  So stage k is done with after slot
+        // 4 k + 3 and stage k + 1 has to be there by then.
+        //
+        // LDS holds 5 operand tiles: both of stage k, both of stage k + 1 and
+        // p of stage k + 2, in turn.  A wave fetches its part of q of stage k + 1,
+        // then of p of stage k + 2, along with its reads of the two halves: a
+        // load waits for its turn, which would hold up products behind it.
+        static_assert(BK == 64 && S == 2 && BP == BQ && NP == 4 && NQ == 4, "5 tiles of equal size");
+        constexpr int TILE = BP * 2 * BK;
+        const bool second = wave >= 4;
+        const int n = (cn - c0 + BK - 1) / BK;
+        lds8_t* const tiles = (lds8_t*)lds;
+        auto slot_end = [&]() __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto fetch_q = [&](int k, int t) __attribute__((always_inline)) {
+            if (k < n)
+#pragma unroll
+                for (int i = 0; i < NQ; i++) fill_q(c0 + k * BK, i, tiles + t * TILE);
+        };
+        auto fetch_p = [&](int k, int t) __attribute__((always_inline)) {
+            if (k < n)
+#pragma unroll
+                for (int i = 0; i < NP; i++) fill_p(c0 + k * BK, i, tiles + t * TILE);
+        };
+        auto landed = [&](int k) __attribute__((always_inline)) {       // stage k + 1; p of stage k + 2 may not be
+            if (k + 2 < n) WM_WAIT_VMCNT(4);
+            else WM_WAIT_VMCNT(0);
+        };
+        auto products = [&]() __attribute__((always_inline)) {
+            __builtin_amdgcn_s_setprio(1);
             multiply();
-            read(1, b);
-            multiply();
-            WM_WAIT_VMCNT(0);                   // this wave's part of the next stage
-            __syncthreads();                    // and its last reads of this one
-            if (c + 2 * BK < cn) {
-                fill(c + 2 * BK, b);
-                tokens(c + 3 * BK);
+            __builtin_amdgcn_s_setprio(0);
+        };
+        if (n > 0) {
+            fetch_p(0, 0);
+            fetch_q(0, 1);
+            fetch_p(1, 2);
+            landed(-1);
+            slot_end();
+            if (second) slot_end();
+            int tp = 0;                                     // tile of p of stage k; q's is the next
+            for (int k = 0; k < n; k++) {
+                const lds8_t *pt = tiles + tp * TILE, *qt = tiles + (tp == 4 ? 0 : tp + 1) * TILE;
+                read(0, pt, qt);
+                fetch_q(k + 1, tp >= 2 ? tp - 2 : tp + 3);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                slot_end();
+                products();
+                slot_end();
+                read(1, pt, qt);
+                fetch_p(k + 2, tp >= 1 ? tp - 1 : tp + 4);
+                if (second) landed(k);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                slot_end();
+                products();
+                if (!second) landed(k);
+                slot_end();
+                tp = tp >= 3 ? tp - 3 : tp + 2;
             }
+            if (!second) slot_end();
+        }
+    } else if (c0 < cn) {
+        auto fill = [&](int c, int b) __attribute__((always_inline)) {
+            lds8_t* dst = (lds8_t*)lds + b * STAGE;
+#pragma unroll
+            for (int i = 0; i < NP; i++) fill_p(c, i, dst);
+#pragma unroll
+            for (int i = 0; i < NQ; i++) fill_q(c, i, dst + PS * 16);
+        };
+#pragma unroll
+        for (int i = 0; i < S - 1; i++) {
+            if (i && c0 + i * BK >= cn) break;
+            fill(c0 + i * BK, i);
+        }
+        int b = 0;
+        for (int c = c0; c < cn; c += BK) {
+            // stages c + BK .. c + (S - 2) BK may still be in flight
+            if (S > 2 && c + (S - 2) * BK < cn) WM_WAIT_VMCNT((S - 2) * (NP + NQ));
+            else WM_WAIT_VMCNT(0);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (c + (S - 1) * BK < cn) fill(c + (S - 1) * BK, b == 0 ? S - 1 : b - 1);
+            const lds8_t* pt = (const lds8_t*)lds + b * STAGE;
+#pragma unroll
+            for (int h = 0; h < BK / 32; h++) {
+                read(h, pt, pt + PS * 16);
+                multiply();
+            }
+            b = b == S - 1 ? 0 : b + 1;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the epilogue writes over the last stage
+    }
+    if (sums) store_db<FQ>(a, e, part, q0 + wq * (BQ / WQ), lane, sum);
+    if (DIR == DW && !a.dw) return;
+    store_tile<BF, DIR, FP, FQ, PH>(a, e, part, p0 + (gated ? wp * (BP / WP / 2) : wp * (BP / WP)), q0 + wq * (BQ / WQ), qn, outs, lane, acc,
+                                    (lf32_t*)lds + wave * epilogue_floats<FP, FQ, PH>());
+}
+
+// ------------------------------------------------------------------ joining parts
+
+// Adds the parts' sums in order and finishes the outputs: one thread per 8 of
+// them.  Rows of no group are left out.
+template <bool BF, int DIR> __global__ __launch_bounds__(256) void k_join(const ProductArgs a) {
+    const bool gated = DIR == FWD && a.act == WM_ACT_SWIGLU;
+    const int width = DIR == FWD ? a.out : a.in, outs = gated ? width / 2 : width;
+    const int rows = DIR == DW ? a.E * a.out : a.rows;
+    const uint32_t per = (outs + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t r = i / per;
+    if (r >= rows) return;
+    const int p = (int)(i - r * per) * 8, n = outs - p;
+    int e = 0, q = (int)r;
+    if (DIR == DW) {
+        e = q / a.out;
+        q -= e * a.out;
+        if (a.db && p == 0) {
+            float s = 0.0f;
+            for (int k = 0; k < a.split; k++) s += a.part_db[(int64_t)k * rows + r];
+            a.db[r] = s;
+        }
+        if (!a.dw) return;
+    } else if (a.offsets) {
+        if (q < a.offsets[0] || q >= a.offsets[a.E]) return;
+        int hi = a.E;                   // offsets[e] <= q < offsets[hi]
+        while (hi - e > 1) {
+            const int mid = (e + hi) / 2;
+            if (a.offsets[mid] <= q) e = mid;
+            else hi = mid;
         }
     }
-    if (sums) store_db<FQ>(a, e, q0 + wq * (BQ / WQ), lane, sum);
-    if (DIR == DW && !a.dw) return;
-    store_tile<BF, DIR, FP, FQ, PH>(a, e, p0 + (gated ? wp * (BP / WP / 2) : wp * (BP / WP)), q0 + wq * (BQ / WQ), qn, outs, lane, acc,
-                                    (lf32_t*)lds + wave * epilogue_floats<FP, FQ, PH>());
+    float z[8] = {0, 0, 0, 0, 0, 0, 0, 0}, up[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8];
+#pragma unroll 4
+    for (int k = 0; k < a.split; k++) {
+        const float* s = a.part + ((int64_t)k * rows + r) * width + p;
+        getf8(s, n, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) z[j] += v[j];
+        if (gated) {
+            getf8(s + outs, n, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) up[j] += v[j];
+        }
+    }
+    store8<BF, DIR>(a, e, q, p, outs, z, up);
+}
+
+// ------------------------------------------------------------------ few rows
+
+// 8 values that nobody reads again soon; no alignment needed.
+typedef s16x8 s16x8u __attribute__((aligned(2)));
+WM_DEV s16x8 stream8(const uint16_t* p) {
+#ifdef NONT
+    s16x8 v; __builtin_memcpy(&v, p, 16); return v;
+#else
+    return __builtin_nontemporal_load((const s16x8u*)p);
+#endif
+}
+
+// Forward product of up to 16 * MT rows per group, bound by streaming W once.
+// A workgroup takes 16 rows of W (SwiGLU: 8 gate rows and their up rows) and
+// all of the contraction, split over its waves in contiguous parts, so enough
+// workgroups exist without sums across them.  W goes from memory straight
+// into the operand registers, B loads of 1 KB in flight per wave; x is
+// read from the caches.  The waves' sums meet in LDS, in wave order.
+// No alignment is assumed: only the last step of 32 may be partial.
+template <bool BF, int MT, int NW, int B> __global__ __launch_bounds__(64 * NW) void k_product_few(const ProductArgs a) {
+    constexpr int ROW = 20;             // floats per row of sums, 16 used
+    __shared__ __attribute__((aligned(16))) float red[NW * MT * 16 * ROW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, l = lane & 15;
+    const bool gated = a.act == WM_ACT_SWIGLU;
+    const int outs = gated ? a.out / 2 : a.out, cols = gated ? 8 : 16, nP = (outs + cols - 1) / cols;
+    const GroupTile t = find_tile(a.offsets, a.E, a.rows, 16 * MT, blockIdx.x / nP);
+    if (t.e < 0) return;
+    const int p0 = (int)(blockIdx.x % nP) * cols, q0 = t.start + t.tile * 16 * MT, qn = t.start + t.n;
+
+    const int o = min(p0 + (gated ? l & 7 : l), outs - 1);
+    const uint16_t* wrow = a.w + (int64_t)t.e * a.w_stride + (int64_t)(gated && (l & 8) ? outs + o : o) * a.ldw + 8 * g;
+    const uint16_t* xrow[MT];
+    bool live[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        const int q = q0 + 16 * m + l;
+        const int r = q < qn ? (a.token ? a.token[q] : q) : -1;
+        live[m] = (uint32_t)r < (uint32_t)a.x_rows;
+        xrow[m] = a.x + (int64_t)(live[m] ? r : 0) * a.ldx + 8 * g;
+    }
+    f32x4 acc[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; m++) acc[m][0] = acc[m][1] = (f32x4)0.0f;
+    const int steps = (a.in + 31) / 32, per = (steps + NW - 1) / NW, s1 = min((wave + 1) * per, steps);
+    int s = wave * per;
+    auto batch = [&](auto n) __attribute__((always_inline)) {
+        constexpr int N = decltype(n)::value;
+        s16x8 wv[N], xv[MT][N];
+#pragma unroll
+        for (int i = 0; i < N; i++) wv[i] = stream8(wrow + 32 * (s + i));
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+#pragma unroll
+            for (int i = 0; i < N; i++) xv[m][i] = (s16x8)0;
+            if (live[m])
+#pragma unroll
+                for (int i = 0; i < N; i++) __builtin_memcpy(&xv[m][i], xrow[m] + 32 * (s + i), 16);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int m = 0; m < MT; m++) acc[m][i & 1] = mfma<BF>(wv[i], xv[m][i], acc[m][i & 1]);
+        s += N;
+    };
+    const int full = min(s1, a.in / 32);
+    while (s + B <= full) batch(std::integral_constant<int, B>());
+    while (s + 4 <= full) batch(std::integral_constant<int, 4>());
+    while (s < full) batch(std::integral_constant<int, 1>());
+    if (s < s1) {
+        const int c = 32 * s, n = a.in - c - 8 * g;
+        const uint4 wt = load8(wrow + c, n);
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const uint4 xt = load8(xrow[m] + c, live[m] ? n : 0);
+            acc[m][0] = mfma<BF>(__builtin_bit_cast(s16x8, wt), __builtin_bit_cast(s16x8, xt), acc[m][0]);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++) *(f32x4*)&red[((wave * MT + m) * 16 + l) * ROW + 4 * g] = acc[m][0] + acc[m][1];
+    __syncthreads();
+    for (int k = threadIdx.x; k < MT * 16 * cols; k += 64 * NW) {
+        const int r = k / cols, j = k % cols, q = q0 + r, p = p0 + j;
+        if (q >= qn || p >= outs) continue;
+        float z = 0.0f, u = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            z += red[(w * MT * 16 + r) * ROW + j];
+            if (gated) u += red[(w * MT * 16 + r) * ROW + 8 + j];
+        }
+        store_one<BF>(a, t.e, q, p, outs, z, u);
+    }
 }
 
 // ------------------------------------------------------------------ launch
@@ -587,16 +876,20 @@ static int64_t row_tiles(int64_t rows, int64_t E, int bq, bool grouped) {
     return std::min(rows, rows / bq + E);
 }
 
-template <int DIR, int BP, int BQ, int WP, int WQ, bool DMA> static int run(const ProductArgs& a, int64_t qtiles, hipStream_t s) {
+template <int DIR, int BP, int BQ, int WP, int WQ, int S, int KB = 64> static int run(const ProductArgs& a, int64_t qtiles, hipStream_t s) {
     const bool gated = DIR == FWD && a.act == WM_ACT_SWIGLU;
     const int outs = DIR == FWD ? (gated ? a.out / 2 : a.out) : a.in, cols = gated ? BP / 2 : BP;
-    const int64_t blocks = qtiles * ((outs + cols - 1) / cols);
+    const int64_t blocks = qtiles * ((outs + cols - 1) / cols) * a.split;
     if (blocks == 0) return 0;
     if (blocks > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
     void (*k)(const ProductArgs);
-    if constexpr (DMA) k = a.bf16 ? k_product_dma<true, DIR, BP, BQ, WP, WQ> : k_product_dma<false, DIR, BP, BQ, WP, WQ>;
+    if constexpr (S > 0) k = a.bf16 ? k_product_dma<true, DIR, BP, BQ, WP, WQ, S, KB> : k_product_dma<false, DIR, BP, BQ, WP, WQ, S, KB>;
     else k = a.bf16 ? k_product<true, DIR, BP, BQ, WP, WQ> : k_product<false, DIR, BP, BQ, WP, WQ>;
     hipLaunchKernelGGL(k, dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
+    if (a.split > 1) {
+        const int64_t rows = DIR == DW ? (int64_t)a.E * a.out : a.rows;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(a.bf16 ? k_join<true, DIR> : k_join<false, DIR>), dim3((uint32_t)((rows * ((outs + 7) / 8) + 255) / 256)), dim3(256), 0, s, a);
+    }
     return (int)hipGetLastError();
 }
 
@@ -611,22 +904,80 @@ template <int DIR> static bool whole_chunks(const ProductArgs& a) {
 template <int DIR> static int run_rows(const ProductArgs& a, hipStream_t s) {
     const bool grouped = a.offsets != nullptr;
     const int64_t per = a.rows / std::max(a.E, 1);
+    const_cast<ProductArgs&>(a).split = 1;
     if (!whole_chunks<DIR>(a)) {
-        if (per <= 32) return run<DIR, 128, 32, 4, 1, false>(a, row_tiles(a.rows, a.E, 32, grouped), s);
-        return run<DIR, 128, 128, 2, 2, false>(a, row_tiles(a.rows, a.E, 128, grouped), s);
+        if (per <= 32) return run<DIR, 128, 32, 4, 1, 0>(a, row_tiles(a.rows, a.E, 32, grouped), s);
+        return run<DIR, 128, 128, 2, 2, 0>(a, row_tiles(a.rows, a.E, 128, grouped), s);
     }
-    if (per <= 32) return run<DIR, 128, 32, 4, 1, true>(a, row_tiles(a.rows, a.E, 32, grouped), s);
-    if (per <= 128) return run<DIR, 128, 128, 2, 2, true>(a, row_tiles(a.rows, a.E, 128, grouped), s);
-    return run<DIR, 256, 256, 2, 4, true>(a, row_tiles(a.rows, a.E, 256, grouped), s);
+    const int cfg = getenv("CFG") ? atoi(getenv("CFG")) : 0;
+    static float* buf = nullptr;
+    const int split = getenv("SPLIT") ? atoi(getenv("SPLIT")) : 1;
+    ProductArgs b = a;
+    b.split = split;
+    if (split > 1) { if (!buf) { if (hipMalloc(&buf, 2ll << 30) != hipSuccess) return 1; } b.part = buf; }
+#define RUN(BP, BQ, ...) return run<DIR, BP, BQ, __VA_ARGS__>(b, row_tiles(a.rows, a.E, BQ, grouped), s)
+    switch (cfg) {
+    case 0: RUN(256, 256, 2, 4, 2);
+    case 1: RUN(128, 128, 2, 2, 2);
+    case 2: RUN(128, 64, 2, 2, 3);
+    case 3: RUN(128, 32, 4, 1, 3);
+    case 4: RUN(128, 32, 4, 1, 4);
+    case 5: RUN(64, 32, 4, 1, 4);
+    case 6: RUN(64, 16, 2, 1, 4);
+    case 7: RUN(128, 16, 2, 1, 4);
+    case 8: RUN(64, 64, 2, 2, 4);
+    case 14: RUN(128, 128, 2, 2, 4, 32);
+    default: RUN(32, 16, 1, 1, 4);
+    }
 }
 
-int launch_product(const ProductArgs& a, hipStream_t s) { return run_rows<FWD>(a, s); }
+template <int MT, int NW, int B> static int run_few(const ProductArgs& a, hipStream_t s) {
+    const bool gated = a.act == WM_ACT_SWIGLU;
+    const int outs = gated ? a.out / 2 : a.out, cols = gated ? 8 : 16;
+    const int64_t blocks = row_tiles(a.rows, a.E, 16 * MT, a.offsets != nullptr) * ((outs + cols - 1) / cols);
+    if (blocks > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
+    const auto k = a.bf16 ? k_product_few<true, MT, NW, B> : k_product_few<false, MT, NW, B>;
+    hipLaunchKernelGGL(k, dim3((uint32_t)blocks), dim3(64 * NW), 0, s, a);
+    return (int)hipGetLastError();
+}
+
+int launch_product(const ProductArgs& a, hipStream_t s) {
+    const int64_t per = a.rows / std::max(a.E, 1);
+    const int few = getenv("FEW") ? atoi(getenv("FEW")) : 16;
+    const int nw = getenv("NW") ? atoi(getenv("NW")) : 0;
+    if (per <= few) {
+        if (per <= 16) {
+        if (nw == 0) return run_few<1, 1, 16>(a, s);
+        if (nw == 1) return run_few<1, 2, 16>(a, s);
+        if (nw == 2) return run_few<1, 4, 16>(a, s);
+        if (nw == 3) return run_few<1, 8, 16>(a, s);
+        if (nw == 4) return run_few<1, 2, 8>(a, s);
+        if (nw == 5) return run_few<1, 4, 8>(a, s);
+        if (nw == 6) return run_few<1, 8, 8>(a, s);
+        } else {
+        if (nw == 1) return run_few<2, 2, 16>(a, s);
+        if (nw == 2) return run_few<2, 4, 16>(a, s);
+        if (nw == 3) return run_few<2, 8, 16>(a, s);
+        if (nw == 4) return run_few<2, 2, 8>(a, s);
+        if (nw == 5) return run_few<2, 4, 8>(a, s);
+        if (nw == 6) return run_few<2, 8, 8>(a, s);
+        }
+    }
+    return run_rows<FWD>(a, s);
+}
 int launch_product_dx(const ProductArgs& a, hipStream_t s) { return run_rows<DX>(a, s); }
 int launch_product_dw(const ProductArgs& args, hipStream_t s) {
     ProductArgs a = args;
     if (!a.dw) a.in = 1;        // db alone: one tile of p
-    if (!whole_chunks<DW>(a)) return run<DW, 128, 128, 2, 2, false>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
-    return run<DW, 256, 256, 2, 4, true>(a, (int64_t)a.E * ((a.out + 255) / 256), s);
+    a.split = 1;
+    if (!whole_chunks<DW>(a)) return run<DW, 128, 128, 2, 2, 0>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
+    const int cfg = getenv("CFG") ? atoi(getenv("CFG")) : 0;
+    switch (cfg) {
+    case 1: return run<DW, 128, 128, 2, 2, 2>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
+    case 14: return run<DW, 128, 128, 2, 2, 4, 32>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
+    case 2: return run<DW, 128, 64, 2, 2, 3>(a, (int64_t)a.E * ((a.out + 63) / 64), s);
+    default: return run<DW, 256, 256, 2, 4, 2>(a, (int64_t)a.E * ((a.out + 255) / 256), s);
+    }
 }
 
 }  // namespace wm
