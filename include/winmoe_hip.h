@@ -313,18 +313,23 @@ typedef struct wm_product_desc {
     int64_t ldy;
     void* pre;               /* [rows][out]: receives x W^T + bias before the activation, or NULL */
     int64_t ld_pre;
+    const void* dz;          /* backward: gradient of x W^T + bias, [rows][out] */
+    int64_t ld_dz;
 } wm_product_desc;
 
-/* Bytes of workspace a call may use (0: none; < 0: bad descriptor).  backward:
- * 0 for wm_product, 1 for wm_product_backward.  One call at a time may use a
- * workspace; it needs no clearing and keeps nothing between calls. */
+/* Bytes of workspace that a call with this descriptor needs (0: none; < 0: bad
+ * descriptor); backward: 0 for wm_product, 1 for wm_product_backward.  It holds
+ * copies of operands whose rows are odd or unaligned, and sums of parts of a
+ * long contraction where there are few outputs.  256-byte aligned; one call at
+ * a time may use a workspace; it needs no clearing and keeps nothing between
+ * calls. */
 int64_t wm_product_workspace_size(const wm_product_desc* d, int backward);
 
 /* y[r] = act(W_e x[token[r]] + bias_e) + residual[r] for every row r of every
  * group e. */
 int wm_product(const wm_product_desc* d, void* ws, int64_t ws_bytes, void* stream);
 
-/* Gradients of z = x W^T + bias, given dz [rows][out] (dtype):
+/* Gradients of z = x W^T + bias, given d->dz:
  *   dx[r] = W_e^T dz[r]             [rows][in] (dtype), one row per row of dz: with
  *                                   token, wm_combine_rows sums them per row of x
  *   dw[e] = sum_r dz[r] x[token[r]]^T  [n_groups][out][in] dense, dw_type dtype or WM_F32
@@ -333,8 +338,8 @@ int wm_product(const wm_product_desc* d, void* ws, int64_t ws_bytes, void* strea
  * sums run in a fixed order: the same call gives the same bits.  d->y, bias,
  * residual and pre are not used and d->act must be WM_ACT_NONE (see
  * wm_act_backward for the step before). */
-int wm_product_backward(const wm_product_desc* d, const void* dz, int64_t ld_dz, void* dx, int64_t ld_dx, void* dw,
-                        int dw_type, float* db, void* ws, int64_t ws_bytes, void* stream);
+int wm_product_backward(const wm_product_desc* d, void* dx, int64_t ld_dx, void* dw, int dw_type, float* db, void* ws,
+                        int64_t ws_bytes, void* stream);
 
 /* dz = act'(pre) * dy: dy [rows][cols], pre and dz [rows][cols] or, with
  * WM_ACT_SWIGLU, [rows][2 cols] (gate half, up half).  dz may be pre. */

@@ -45,13 +45,17 @@ def test_product_refuses(lib, kw):
 def test_product_workspace_and_backward_refuse(lib, kw):
     d = desc(**kw)
     assert lib.wm_product_workspace_size(C.byref(d), 0) < 0
-    assert lib.wm_product_backward(C.byref(d), 64, 16, 64, 8, None, 0, None, None, 0, None) == -2
+    d.dz, d.ld_dz = 64, 16
+    assert lib.wm_product_workspace_size(C.byref(d), 1) < 0
+    assert lib.wm_product_backward(C.byref(d), 64, 8, None, 0, None, None, 0, None) == -2
 
 
 def test_product_backward_refuses(lib):
     d = desc()
-    call = lambda d, dz=64, ldz=16, dx=None, ldx=8, dw=None, wt=30, db=None: lib.wm_product_backward(
-        C.byref(d), dz, ldz, dx, ldx, dw, wt, db, None, 0, None)
+    def call(d, dz=64, ldz=16, dx=None, ldx=8, dw=None, wt=30, db=None):
+        d.dz, d.ld_dz = dz, ldz
+        return lib.wm_product_backward(C.byref(d), dx, ldx, dw, wt, db, None, 0, None)
+
     assert call(desc(act=1), dx=64) == -2                    # the activation's gradient is a step of its own
     assert call(d, dz=None, dx=64) == -2
     assert call(d, dz=65, dx=64) == -2
@@ -105,7 +109,7 @@ def test_empty_calls_return_at_once(lib):
 
 def test_descriptor_is_as_long_as_the_headers(lib):
     from winmoe_amd import _lib
-    assert C.sizeof(_lib.ProductDesc) == 8 * 4 + 14 * 8
+    assert C.sizeof(_lib.ProductDesc) == 8 * 4 + 16 * 8
 
 
 def test_python_refuses_host_tensors():

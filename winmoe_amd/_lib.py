@@ -60,7 +60,7 @@ class ProductDesc(C.Structure):
         ("offsets", _vp), ("token", _vp),
         ("x", _vp), ("ldx", _i64), ("w", _vp), ("ldw", _i64), ("w_stride", _i64),
         ("bias", _vp), ("residual", _vp), ("ld_residual", _i64),
-        ("y", _vp), ("ldy", _i64), ("pre", _vp), ("ld_pre", _i64),
+        ("y", _vp), ("ldy", _i64), ("pre", _vp), ("ld_pre", _i64), ("dz", _vp), ("ld_dz", _i64),
     ]
 
 
@@ -113,8 +113,7 @@ SIGNATURES = {
     "wm_expert_workspace_size": (_i64, [C.c_int, C.c_int]),
     "wm_product_workspace_size": (_i64, [_vp, C.c_int]),
     "wm_product": (C.c_int, [_vp, _vp, _i64, _vp]),
-    "wm_product_backward": (C.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, C.c_int, _vp, _vp, _i64,
-                                      _vp]),
+    "wm_product_backward": (C.c_int, [_vp, _vp, _i64, _vp, C.c_int, _vp, _vp, _i64, _vp]),
     "wm_act_backward": (C.c_int, [C.c_int, C.c_int, _i64, C.c_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "wm_group_by_expert": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp]),
     "wm_combine_rows": (C.c_int, [C.c_int, _vp, _i64, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _i64, _vp,

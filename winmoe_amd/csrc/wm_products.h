@@ -49,9 +49,11 @@ struct ProductArgs {
     float *part, *part_db;
 };
 
-int launch_product(const ProductArgs& a, hipStream_t s);
-int launch_product_dx(const ProductArgs& a, hipStream_t s);
-int launch_product_dw(const ProductArgs& a, hipStream_t s);
+// Bytes of workspace that a direction (backward: DX and DW together) uses.
+int64_t product_workspace(const ProductArgs& a, bool backward);
+// ws holds product_workspace() bytes, 256-byte aligned.
+int launch_product(const ProductArgs& a, uint8_t* ws, hipStream_t s);
+int launch_product_backward(const ProductArgs& a, uint8_t* ws, hipStream_t s);     // dx, dw, db: those not NULL
 
 int launch_group(const int32_t* ids, int T, int K, int E, int32_t* offsets, int32_t* token, int32_t* row,
                  hipStream_t s);

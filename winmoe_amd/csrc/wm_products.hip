@@ -18,8 +18,8 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
-#include <stdlib.h>
 
 #include "../../include/winmoe_hip.h"
 #include "wm_act.h"
@@ -123,16 +123,17 @@ WM_DEV GroupTile find_tile(const int32_t* __restrict__ offsets, int E, int rows,
 }
 
 // Workgroup -> tile.  Workgroups go round the 8 XCDs, so each XCD takes a
-// contiguous run of tiles, in blocks of 8 row tiles times all column tiles:
+// contiguous run of tiles, in blocks of 4 row tiles times all column tiles:
 // what runs on an XCD at once shares rows and columns in its L2.
 struct TileId {
     int p, q;
 };
+constexpr int TILE_ROWS = 4;
 WM_DEV TileId tile_id(int block, int blocks, int nP) {
     const int per = blocks / 8, rest = blocks % 8, xcd = block % 8;
     const int t = xcd * per + min(xcd, rest) + block / 8;
-    const int q8 = t / (8 * nP), nq = min(8, blocks / nP - 8 * q8), in = t - q8 * 8 * nP;
-    return {in / nq, 8 * q8 + in % nq};
+    const int qb = t / (TILE_ROWS * nP), nq = min(TILE_ROWS, blocks / nP - TILE_ROWS * qb), in = t - qb * TILE_ROWS * nP;
+    return {in / nq, TILE_ROWS * qb + in % nq};
 }
 
 // ------------------------------------------------------------------ LDS tiles
@@ -313,6 +314,7 @@ template <int FQ> WM_DEV void store_db(const ProductArgs& a, int e, int part, in
 template <bool BF, int DIR, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     constexpr int NT = 64 * WP * WQ, FP = BP / WP / 16, FQ = BQ / WQ / 16;
+    static_assert(DIR != FWD || FP % 2 == 0, "SwiGLU's gate and up meet in a wave");
     constexpr bool PC = DIR == FWD, QC = DIR != DW;         // operand's rows run along the contraction
     using PT = typename std::conditional<PC, AlongC<BP, BK>, AcrossC<BP, BK>>::type;
     using QT = typename std::conditional<QC, AlongC<BQ, BK>, AcrossC<BQ, BK>>::type;
@@ -480,6 +482,7 @@ static __device__ __attribute__((aligned(16))) uint16_t zero_chunk[8];
 template <bool BF, int DIR, int BP, int BQ, int WP, int WQ, int S, int BK>
 __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs a) {
     constexpr int NT = 64 * WP * WQ, FP = BP / WP / 16, FQ = BQ / WQ / 16;
+    static_assert(DIR != FWD || FP % 2 == 0, "SwiGLU's gate and up meet in a wave");
     constexpr bool PC = DIR == FWD, QC = DIR != DW;
     using PT = typename std::conditional<PC, AlongC<BP, BK>, AcrossC<BP, BK>>::type;
     using QT = typename std::conditional<QC, AlongC<BQ, BK>, AcrossC<BQ, BK>>::type;
@@ -777,110 +780,229 @@ template <bool BF, int DIR> __global__ __launch_bounds__(256) void k_join(const 
 
 // ------------------------------------------------------------------ few rows
 
-// 8 values that nobody reads again soon; no alignment needed.
-typedef s16x8 s16x8u __attribute__((aligned(2)));
-WM_DEV s16x8 stream8(const uint16_t* p) {
-#ifdef NONT
-    s16x8 v; __builtin_memcpy(&v, p, 16); return v;
-#else
-    return __builtin_nontemporal_load((const s16x8u*)p);
-#endif
-}
-
-// Forward product of up to 16 * MT rows per group, bound by streaming W once.
-// A workgroup takes 16 rows of W (SwiGLU: 8 gate rows and their up rows) and
-// all of the contraction, split over its waves in contiguous parts, so enough
+// Forward product of up to 16 rows per tile, bound by streaming W once.  A
+// workgroup takes 16 rows of W (SwiGLU: 8 gate rows and their up rows) and all
+// of the contraction, split over its waves in contiguous parts, so enough
 // workgroups exist without sums across them.  W goes from memory straight
-// into the operand registers, B loads of 1 KB in flight per wave; x is
-// read from the caches.  The waves' sums meet in LDS, in wave order.
-// No alignment is assumed: only the last step of 32 may be partial.
-template <bool BF, int MT, int NW, int B> __global__ __launch_bounds__(64 * NW) void k_product_few(const ProductArgs a) {
+// into the operand registers, 8 loads of 1 KB in flight per wave; x is read
+// from the caches.  The waves' sums meet in LDS, in wave order.  No alignment
+// is assumed: only the last step of 32 may be partial.
+template <bool BF, int NW> __global__ __launch_bounds__(64 * NW) void k_product_few(const ProductArgs a) {
     constexpr int ROW = 20;             // floats per row of sums, 16 used
-    __shared__ __attribute__((aligned(16))) float red[NW * MT * 16 * ROW];
+    __shared__ __attribute__((aligned(16))) float red[NW * 16 * ROW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, l = lane & 15;
     const bool gated = a.act == WM_ACT_SWIGLU;
     const int outs = gated ? a.out / 2 : a.out, cols = gated ? 8 : 16, nP = (outs + cols - 1) / cols;
-    const GroupTile t = find_tile(a.offsets, a.E, a.rows, 16 * MT, blockIdx.x / nP);
+    const GroupTile t = find_tile(a.offsets, a.E, a.rows, 16, blockIdx.x / nP);
     if (t.e < 0) return;
-    const int p0 = (int)(blockIdx.x % nP) * cols, q0 = t.start + t.tile * 16 * MT, qn = t.start + t.n;
+    const int p0 = (int)(blockIdx.x % nP) * cols, q0 = t.start + t.tile * 16, qn = t.start + t.n;
 
-    const int o = min(p0 + (gated ? l & 7 : l), outs - 1);
+    const int o = min(p0 + (gated ? l & 7 : l), outs - 1), q = q0 + l;
     const uint16_t* wrow = a.w + (int64_t)t.e * a.w_stride + (int64_t)(gated && (l & 8) ? outs + o : o) * a.ldw + 8 * g;
-    const uint16_t* xrow[MT];
-    bool live[MT];
-#pragma unroll
-    for (int m = 0; m < MT; m++) {
-        const int q = q0 + 16 * m + l;
-        const int r = q < qn ? (a.token ? a.token[q] : q) : -1;
-        live[m] = (uint32_t)r < (uint32_t)a.x_rows;
-        xrow[m] = a.x + (int64_t)(live[m] ? r : 0) * a.ldx + 8 * g;
-    }
-    f32x4 acc[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; m++) acc[m][0] = acc[m][1] = (f32x4)0.0f;
+    const int r = q < qn ? (a.token ? a.token[q] : q) : -1;
+    const bool live = (uint32_t)r < (uint32_t)a.x_rows;
+    const uint16_t* xrow = a.x + (int64_t)(live ? r : 0) * a.ldx + 8 * g;
+    f32x4 acc[2] = {(f32x4)0.0f, (f32x4)0.0f};
     const int steps = (a.in + 31) / 32, per = (steps + NW - 1) / NW, s1 = min((wave + 1) * per, steps);
     int s = wave * per;
     auto batch = [&](auto n) __attribute__((always_inline)) {
         constexpr int N = decltype(n)::value;
-        s16x8 wv[N], xv[MT][N];
+        s16x8 wv[N], xv[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) wv[i] = stream8(wrow + 32 * (s + i));
+        for (int i = 0; i < N; i++) __builtin_memcpy(&wv[i], wrow + 32 * (s + i), 16);
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
+        for (int i = 0; i < N; i++) xv[i] = (s16x8)0;
+        if (live)
 #pragma unroll
-            for (int i = 0; i < N; i++) xv[m][i] = (s16x8)0;
-            if (live[m])
+            for (int i = 0; i < N; i++) __builtin_memcpy(&xv[i], xrow + 32 * (s + i), 16);
 #pragma unroll
-                for (int i = 0; i < N; i++) __builtin_memcpy(&xv[m][i], xrow[m] + 32 * (s + i), 16);
-        }
-#pragma unroll
-        for (int i = 0; i < N; i++)
-#pragma unroll
-            for (int m = 0; m < MT; m++) acc[m][i & 1] = mfma<BF>(wv[i], xv[m][i], acc[m][i & 1]);
+        for (int i = 0; i < N; i++) acc[i & 1] = mfma<BF>(wv[i], xv[i], acc[i & 1]);
         s += N;
     };
     const int full = min(s1, a.in / 32);
-    while (s + B <= full) batch(std::integral_constant<int, B>());
+    while (s + 8 <= full) batch(std::integral_constant<int, 8>());
     while (s + 4 <= full) batch(std::integral_constant<int, 4>());
     while (s < full) batch(std::integral_constant<int, 1>());
     if (s < s1) {
         const int c = 32 * s, n = a.in - c - 8 * g;
-        const uint4 wt = load8(wrow + c, n);
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const uint4 xt = load8(xrow[m] + c, live[m] ? n : 0);
-            acc[m][0] = mfma<BF>(__builtin_bit_cast(s16x8, wt), __builtin_bit_cast(s16x8, xt), acc[m][0]);
-        }
+        const uint4 wt = load8(wrow + c, n), xt = load8(xrow + c, live ? n : 0);
+        acc[0] = mfma<BF>(__builtin_bit_cast(s16x8, wt), __builtin_bit_cast(s16x8, xt), acc[0]);
     }
-#pragma unroll
-    for (int m = 0; m < MT; m++) *(f32x4*)&red[((wave * MT + m) * 16 + l) * ROW + 4 * g] = acc[m][0] + acc[m][1];
+    *(f32x4*)&red[(wave * 16 + l) * ROW + 4 * g] = acc[0] + acc[1];
     __syncthreads();
-    for (int k = threadIdx.x; k < MT * 16 * cols; k += 64 * NW) {
-        const int r = k / cols, j = k % cols, q = q0 + r, p = p0 + j;
-        if (q >= qn || p >= outs) continue;
+    for (int k = threadIdx.x; k < 16 * cols; k += 64 * NW) {
+        const int row = k / cols, j = k % cols;
+        if (q0 + row >= qn || p0 + j >= outs) continue;
         float z = 0.0f, u = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            z += red[(w * MT * 16 + r) * ROW + j];
-            if (gated) u += red[(w * MT * 16 + r) * ROW + 8 + j];
+            z += red[(w * 16 + row) * ROW + j];
+            if (gated) u += red[(w * 16 + row) * ROW + 8 + j];
         }
-        store_one<BF>(a, t.e, q, p, outs, z, u);
+        store_one<BF>(a, t.e, q0 + row, p0 + j, outs, z, u);
     }
+}
+
+// ------------------------------------------------------------------ repacking
+
+// Copies rows into rows of `ld` values, zeros behind the first `cols`: makes an
+// operand whose rows are odd or unaligned fit for 16-byte chunks.
+__global__ __launch_bounds__(256) void k_repack(const uint16_t* __restrict__ src, int64_t ld_src, int64_t stride_src, int rows,
+                                                int cols, uint16_t* __restrict__ dst, int ld, int64_t stride_dst) {
+    const uint32_t per = ld / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / per;
+    if (r >= rows) return;
+    const int c = (int)(i - r * per) * 8;
+    const uint4 v = load8(src + blockIdx.y * stride_src + r * ld_src + c, cols - c);
+    *(uint4*)(dst + blockIdx.y * stride_dst + r * ld + c) = v;
 }
 
 // ------------------------------------------------------------------ launch
 
-// Upper bound of the tiles of bq rows that `rows` rows in E groups can make.
-static int64_t row_tiles(int64_t rows, int64_t E, int bq, bool grouped) {
-    if (!grouped) return (rows + bq - 1) / bq;
-    return std::min(rows, rows / bq + E);
+// How a product is run.  The tile kernels' times are estimated from their own
+// measurements (bf16, in 64 stages): `alone` is what a stage of 64 steps takes
+// with one workgroup on a CU, `share` what it adds to a CU that is full, both
+// in us.
+enum Kernel : int { ANY128, ANY32, FEW, T256, T128, T128x64, T128x32, T64, T64x32, T64x16 };
+struct TileCost {
+    Kernel k;
+    int bp, bq, resident;
+    float alone, share;
+};
+static constexpr TileCost kTiles[] = {
+    {T256, 256, 256, 1, 1.40f, 1.65f}, {T128, 128, 128, 2, 0.70f, 0.54f},  {T128x64, 128, 64, 2, 0.58f, 0.36f},
+    {T128x32, 128, 32, 2, 0.46f, 0.33f}, {T64, 64, 64, 2, 0.40f, 0.27f},   {T64x32, 64, 32, 3, 0.34f, 0.20f},
+    {T64x16, 64, 16, 4, 0.34f, 0.15f},
+};
+struct Plan {
+    Kernel k;
+    int split;
+};
+
+static int columns(const ProductArgs& a, int dir) {      // of the result, and of an output tile for SwiGLU
+    return dir == FWD ? (a.act == WM_ACT_SWIGLU ? a.out / 2 : a.out) : a.in;
 }
 
-template <int DIR, int BP, int BQ, int WP, int WQ, int S, int KB = 64> static int run(const ProductArgs& a, int64_t qtiles, hipStream_t s) {
+// Upper bound of the tiles of bq rows that `rows` rows in E groups can make.
+static int64_t row_tiles(const ProductArgs& a, int bq) {
+    if (!a.offsets) return (a.rows + bq - 1) / bq;
+    return std::min((int64_t)a.rows, (int64_t)a.rows / bq + a.E);
+}
+
+// The tile and the number of parts with the least estimated time.  The chip is
+// taken as 256 CUs; the rows of a group are taken as even, as the host does not
+// know them.  A split pays a second kernel and the parts' way to memory and
+// back: 3 us and 3 TB/s.
+static Plan plan_tiles(const ProductArgs& a, int dir) {
+    const double groups = a.offsets ? std::max(1.0, std::min((double)a.E, (double)a.rows)) : 1.0, per = a.rows / groups;
+    const int outs = columns(a, dir);
+    const bool gated = dir == FWD && a.act == WM_ACT_SWIGLU;
+    const double steps = dir == FWD ? a.in : dir == DX ? a.out : per;
+    const double stages = std::max(1.0, std::ceil(steps / BK));
+    const double memory = groups * a.in * a.out * 2.0 * (dir == DW ? 1 + a.dw_f32 : 1) / 5.6e6;     // us
+    const double sums = (dir == DW ? (double)a.E * a.out * a.in : (double)a.rows * (dir == FWD ? a.out : a.in)) * 8.0;
+    Plan best{T128, 1};
+    double least = 1e30;
+    for (const TileCost& t : kTiles) {
+        if (dir == DW && t.bp != t.bq) continue;
+        const double p = std::ceil(outs / (double)(gated ? t.bp / 2 : t.bp));
+        const double q = dir == DW ? a.E * std::ceil(a.out / (double)t.bq) : groups > 1 ? groups * (0.5 + std::max(0.5, per / t.bq)) : std::ceil(per / t.bq);
+        for (int s = 1; s <= 16 && s * 2 <= stages + 1; s *= 2) {
+            if (s > 1 && s * sums > 512e6) break;
+            const double n = std::max(1.0, p * q * s / 256), turns = std::max(1.0, n / t.resident);
+            const double work = std::ceil(stages / s) * std::max(t.alone * turns, t.share * n) + 2.0 * turns;
+            const double us = std::max(work, t.bp < 128 ? 1.15 * memory : memory) + (s > 1 ? 3.0 + s * sums / 3e6 : 0.0);
+            if (us < least) {
+                least = us;
+                best = {t.k, s};
+            }
+        }
+    }
+    return best;
+}
+
+// Whether every 16-byte chunk of an operand is aligned and whole.
+static bool chunks16(const void* p, int64_t ld, int cols) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && cols % 8 == 0; }
+
+// What is copied before the tile kernels: operands of odd or unaligned rows.
+struct Copies {
+    bool x, w, dz;
+};
+static Copies copies(const ProductArgs& a, bool fwd, bool dx, bool dw) {
+    return {(fwd || dw) && !chunks16(a.x, a.ldx, a.in), (fwd || dx) && !(chunks16(a.w, a.ldw, a.in) && a.w_stride % 8 == 0),
+            (dx || dw) && !chunks16(a.dz, a.lddz, a.out)};
+}
+
+// Which kernel takes a forward product (or dx) whose operands need copies, or
+// of few rows.
+//   FEW (forward, up to 16 rows in all, or in a group where copies would be
+//   needed): one launch, 4096 x 4096 weights and one row 9.5 us against 12.4 us
+//   of split tiles; 16 rows and 65536 outputs 128 us against 101 us, so with
+//   many rows only where W is small.
+//   ANY32 (any alignment): groups of under 64 rows whose weights would have to
+//   be copied; they are bound by reading the weights, a copy would read and
+//   write them once more.
+static Plan plan_rows(const ProductArgs& a, int dir) {
+    const int64_t per = a.rows / a.E;
+    const bool odd = dir == FWD ? copies(a, true, false, false).w : copies(a, false, true, false).w;
+    if (dir == FWD && !a.offsets && a.rows <= 16 && (odd || a.rows <= 4 || (int64_t)a.in * a.out <= 1 << 25)) return {FEW, 1};
+    if (odd && a.offsets && per < 64) return {dir == FWD && per <= 2 ? FEW : ANY32, 1};
+    return plan_tiles(a, dir);
+}
+
+struct Layout {
+    int64_t x, w, dz, part, total;
+};
+static int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+static Layout layout(const ProductArgs& a, const Copies& c, int64_t part) {
+    const int64_t in8 = (a.in + 7) / 8 * 8, out8 = (a.out + 7) / 8 * 8;
+    Layout l;
+    l.x = 0;
+    l.w = l.x + (c.x ? up256(2 * in8 * a.x_rows) : 0);
+    l.dz = l.w + (c.w ? up256(2 * in8 * a.out * a.E) : 0);
+    l.part = l.dz + (c.dz ? up256(2 * out8 * a.rows) : 0);
+    l.total = l.part + part;
+    return l;
+}
+static int64_t part_bytes(const ProductArgs& a, int dir, int split) {
+    if (split == 1) return 0;
+    const int64_t n = dir == DW ? (int64_t)a.E * a.out * (a.in + 1) : (int64_t)a.rows * (dir == FWD ? a.out : a.in);
+    return 4 * n * split;
+}
+static bool tiled(const Plan& p) { return p.k >= T256; }
+
+// db without dw takes one column of x.
+static ProductArgs without_dx(const ProductArgs& a) {
+    ProductArgs b = a;
+    if (!b.dw) b.in = 1;
+    return b;
+}
+
+int64_t product_workspace(const ProductArgs& a, bool backward) {
+    if (a.rows == 0) return 0;
+    if (!backward) {
+        const Plan p = plan_rows(a, FWD);
+        return layout(a, tiled(p) ? copies(a, true, false, false) : Copies{}, part_bytes(a, FWD, p.split)).total;
+    }
+    // whichever of dx, dw and db the call asks for
+    ProductArgs b = a;
+    int64_t part = 0;
+    const Plan px = plan_rows(a, DX);
+    part = part_bytes(a, DX, px.split);
+    for (int f32 = 0; f32 < 2; f32++) {
+        b.dw_f32 = f32;
+        part = std::max(part, part_bytes(b, DW, plan_tiles(b, DW).split));
+    }
+    b.in = 1;
+    part = std::max(part, part_bytes(b, DW, plan_tiles(b, DW).split));
+    return layout(a, copies(a, false, tiled(px), true), part).total;
+}
+
+template <int DIR, int BP, int BQ, int WP, int WQ, int S, int KB = 64> static int run(const ProductArgs& a, hipStream_t s) {
     const bool gated = DIR == FWD && a.act == WM_ACT_SWIGLU;
-    const int outs = DIR == FWD ? (gated ? a.out / 2 : a.out) : a.in, cols = gated ? BP / 2 : BP;
+    const int outs = columns(a, DIR), cols = gated ? BP / 2 : BP;
+    const int64_t qtiles = DIR == DW ? (int64_t)a.E * ((a.out + BQ - 1) / BQ) : row_tiles(a, BQ);
     const int64_t blocks = qtiles * ((outs + cols - 1) / cols) * a.split;
-    if (blocks == 0) return 0;
     if (blocks > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
     void (*k)(const ProductArgs);
     if constexpr (S > 0) k = a.bf16 ? k_product_dma<true, DIR, BP, BQ, WP, WQ, S, KB> : k_product_dma<false, DIR, BP, BQ, WP, WQ, S, KB>;
@@ -888,96 +1010,109 @@ template <int DIR, int BP, int BQ, int WP, int WQ, int S, int KB = 64> static in
     hipLaunchKernelGGL(k, dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
     if (a.split > 1) {
         const int64_t rows = DIR == DW ? (int64_t)a.E * a.out : a.rows;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(a.bf16 ? k_join<true, DIR> : k_join<false, DIR>), dim3((uint32_t)((rows * ((outs + 7) / 8) + 255) / 256)), dim3(256), 0, s, a);
+        const int64_t joins = (rows * ((outs + 7) / 8) + 255) / 256;
+        if (joins > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(a.bf16 ? k_join<true, DIR> : k_join<false, DIR>), dim3((uint32_t)joins), dim3(256), 0, s, a);
     }
     return (int)hipGetLastError();
 }
 
-// Whether every 16-byte chunk of the operands is aligned and whole.
-static bool rows16(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
-template <int DIR> static bool whole_chunks(const ProductArgs& a) {
-    if (a.in % 8 || (DIR != FWD && (a.out % 8 || !rows16(a.dz, a.lddz)))) return false;
-    if (DIR != DX && !rows16(a.x, a.ldx)) return false;
-    return DIR == DW || (rows16(a.w, a.ldw) && a.w_stride % 8 == 0);
+template <int DIR> static int run_tiles(const ProductArgs& a, Kernel k, hipStream_t s) {
+    switch (k) {
+    case T256: return run<DIR, 256, 256, 2, 4, 2>(a, s);
+    case T128: return run<DIR, 128, 128, 2, 2, 2>(a, s);
+    case T64: return run<DIR, 64, 64, 2, 2, 4>(a, s);
+    default: break;
+    }
+    if constexpr (DIR != DW) {
+        switch (k) {
+        case T128x64: return run<DIR, 128, 64, 2, 2, 3>(a, s);
+        case T128x32: return run<DIR, 128, 32, 4, 1, 4>(a, s);
+        case T64x32: return run<DIR, 64, 32, 2, 2, 4>(a, s);
+        case T64x16: return run<DIR, 64, 16, 2, 1, 4>(a, s);
+        case ANY32: return run<DIR, 128, 32, 4, 1, 0>(a, s);
+        default: break;
+        }
+    }
+    return (int)hipErrorInvalidValue;
 }
 
-template <int DIR> static int run_rows(const ProductArgs& a, hipStream_t s) {
-    const bool grouped = a.offsets != nullptr;
-    const int64_t per = a.rows / std::max(a.E, 1);
-    const_cast<ProductArgs&>(a).split = 1;
-    if (!whole_chunks<DIR>(a)) {
-        if (per <= 32) return run<DIR, 128, 32, 4, 1, 0>(a, row_tiles(a.rows, a.E, 32, grouped), s);
-        return run<DIR, 128, 128, 2, 2, 0>(a, row_tiles(a.rows, a.E, 128, grouped), s);
-    }
-    const int cfg = getenv("CFG") ? atoi(getenv("CFG")) : 0;
-    static float* buf = nullptr;
-    const int split = getenv("SPLIT") ? atoi(getenv("SPLIT")) : 1;
-    ProductArgs b = a;
-    b.split = split;
-    if (split > 1) { if (!buf) { if (hipMalloc(&buf, 2ll << 30) != hipSuccess) return 1; } b.part = buf; }
-#define RUN(BP, BQ, ...) return run<DIR, BP, BQ, __VA_ARGS__>(b, row_tiles(a.rows, a.E, BQ, grouped), s)
-    switch (cfg) {
-    case 0: RUN(256, 256, 2, 4, 2);
-    case 1: RUN(128, 128, 2, 2, 2);
-    case 2: RUN(128, 64, 2, 2, 3);
-    case 3: RUN(128, 32, 4, 1, 3);
-    case 4: RUN(128, 32, 4, 1, 4);
-    case 5: RUN(64, 32, 4, 1, 4);
-    case 6: RUN(64, 16, 2, 1, 4);
-    case 7: RUN(128, 16, 2, 1, 4);
-    case 8: RUN(64, 64, 2, 2, 4);
-    case 14: RUN(128, 128, 2, 2, 4, 32);
-    default: RUN(32, 16, 1, 1, 4);
-    }
-}
-
-template <int MT, int NW, int B> static int run_few(const ProductArgs& a, hipStream_t s) {
+// 4 waves up to 2048 columns, 8 above: 256 to 512 columns per wave.
+template <int NW> static int run_few(const ProductArgs& a, hipStream_t s) {
     const bool gated = a.act == WM_ACT_SWIGLU;
-    const int outs = gated ? a.out / 2 : a.out, cols = gated ? 8 : 16;
-    const int64_t blocks = row_tiles(a.rows, a.E, 16 * MT, a.offsets != nullptr) * ((outs + cols - 1) / cols);
+    const int outs = columns(a, FWD), cols = gated ? 8 : 16;
+    const int64_t blocks = row_tiles(a, 16) * ((outs + cols - 1) / cols);
     if (blocks > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
-    const auto k = a.bf16 ? k_product_few<true, MT, NW, B> : k_product_few<false, MT, NW, B>;
+    const auto k = a.bf16 ? k_product_few<true, NW> : k_product_few<false, NW>;
     hipLaunchKernelGGL(k, dim3((uint32_t)blocks), dim3(64 * NW), 0, s, a);
     return (int)hipGetLastError();
 }
 
-int launch_product(const ProductArgs& a, hipStream_t s) {
-    const int64_t per = a.rows / std::max(a.E, 1);
-    const int few = getenv("FEW") ? atoi(getenv("FEW")) : 16;
-    const int nw = getenv("NW") ? atoi(getenv("NW")) : 0;
-    if (per <= few) {
-        if (per <= 16) {
-        if (nw == 0) return run_few<1, 1, 16>(a, s);
-        if (nw == 1) return run_few<1, 2, 16>(a, s);
-        if (nw == 2) return run_few<1, 4, 16>(a, s);
-        if (nw == 3) return run_few<1, 8, 16>(a, s);
-        if (nw == 4) return run_few<1, 2, 8>(a, s);
-        if (nw == 5) return run_few<1, 4, 8>(a, s);
-        if (nw == 6) return run_few<1, 8, 8>(a, s);
-        } else {
-        if (nw == 1) return run_few<2, 2, 16>(a, s);
-        if (nw == 2) return run_few<2, 4, 16>(a, s);
-        if (nw == 3) return run_few<2, 8, 16>(a, s);
-        if (nw == 4) return run_few<2, 2, 8>(a, s);
-        if (nw == 5) return run_few<2, 4, 8>(a, s);
-        if (nw == 6) return run_few<2, 8, 8>(a, s);
-        }
-    }
-    return run_rows<FWD>(a, s);
+static int repack(const uint16_t* src, int64_t ld_src, int64_t stride_src, int n, int rows, int cols, uint16_t* dst, hipStream_t s) {
+    const int ld = (cols + 7) / 8 * 8;
+    const int64_t blocks = ((int64_t)rows * (ld / 8) + 255) / 256;
+    if (blocks == 0) return 0;
+    if (blocks > 0x7FFFFFFF || n > 65535) return (int)hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL(k_repack, dim3((uint32_t)blocks, n), dim3(256), 0, s, src, ld_src, stride_src, rows, cols, dst, ld, (int64_t)rows * ld);
+    return (int)hipGetLastError();
 }
-int launch_product_dx(const ProductArgs& a, hipStream_t s) { return run_rows<DX>(a, s); }
-int launch_product_dw(const ProductArgs& args, hipStream_t s) {
-    ProductArgs a = args;
-    if (!a.dw) a.in = 1;        // db alone: one tile of p
-    a.split = 1;
-    if (!whole_chunks<DW>(a)) return run<DW, 128, 128, 2, 2, 0>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
-    const int cfg = getenv("CFG") ? atoi(getenv("CFG")) : 0;
-    switch (cfg) {
-    case 1: return run<DW, 128, 128, 2, 2, 2>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
-    case 14: return run<DW, 128, 128, 2, 2, 4, 32>(a, (int64_t)a.E * ((a.out + 127) / 128), s);
-    case 2: return run<DW, 128, 64, 2, 2, 3>(a, (int64_t)a.E * ((a.out + 63) / 64), s);
-    default: return run<DW, 256, 256, 2, 4, 2>(a, (int64_t)a.E * ((a.out + 255) / 256), s);
+
+// Copies what needs it into the workspace and points the arguments there.
+static int copy_operands(ProductArgs& a, const Copies& c, const Layout& l, uint8_t* ws, hipStream_t s) {
+    const int64_t in8 = (a.in + 7) / 8 * 8, out8 = (a.out + 7) / 8 * 8;
+    if (c.x) {
+        if (int rc = repack(a.x, a.ldx, 0, 1, a.x_rows, a.in, (uint16_t*)(ws + l.x), s)) return rc;
+        a.x = (const uint16_t*)(ws + l.x);
+        a.ldx = in8;
     }
+    if (c.w) {
+        if (int rc = repack(a.w, a.ldw, a.w_stride, a.E, a.out, a.in, (uint16_t*)(ws + l.w), s)) return rc;
+        a.w = (const uint16_t*)(ws + l.w);
+        a.ldw = in8;
+        a.w_stride = in8 * a.out;
+    }
+    if (c.dz) {
+        if (int rc = repack(a.dz, a.lddz, 0, 1, a.rows, a.out, (uint16_t*)(ws + l.dz), s)) return rc;
+        a.dz = (const uint16_t*)(ws + l.dz);
+        a.lddz = out8;
+    }
+    return 0;
+}
+
+int launch_product(const ProductArgs& args, uint8_t* ws, hipStream_t s) {
+    ProductArgs a = args;
+    const Plan p = plan_rows(a, FWD);
+    a.split = p.split;
+    if (p.k == FEW) return a.in <= 2048 ? run_few<4>(a, s) : run_few<8>(a, s);
+    const Copies c = tiled(p) ? copies(a, true, false, false) : Copies{};
+    const Layout l = layout(a, c, 0);
+    if (int rc = copy_operands(a, c, l, ws, s)) return rc;
+    a.part = (float*)(ws + l.part);
+    return run_tiles<FWD>(a, p.k, s);
+}
+
+int launch_product_backward(const ProductArgs& args, uint8_t* ws, hipStream_t s) {
+    ProductArgs a = args;
+    const bool dx = a.dx && a.rows, dw = a.dw || a.db;
+    const Plan px = dx ? plan_rows(a, DX) : Plan{ANY32, 1};
+    const Copies c = copies(a, false, tiled(px), dw && a.rows);
+    const Layout l = layout(a, c, 0);
+    ProductArgs b = a;
+    if (int rc = copy_operands(b, c, l, ws, s)) return rc;
+    b.part = (float*)(ws + l.part);
+    if (dx) {
+        ProductArgs& t = tiled(px) ? b : a;
+        t.split = px.split;
+        if (int rc = run_tiles<DX>(t, px.k, s)) return rc;
+    }
+    if (dw) {
+        ProductArgs t = without_dx(b);
+        const Plan p = a.rows ? plan_tiles(t, DW) : Plan{T128, 1};
+        t.split = p.split;
+        t.part_db = t.part + (int64_t)p.split * t.E * t.out * t.in;
+        return run_tiles<DW>(t, p.k, s);
+    }
+    return 0;
 }
 
 }  // namespace wm

@@ -37,7 +37,27 @@ int check_desc(const wm_product_desc* d) {
     return WM_OK;
 }
 
-ProductArgs common(const wm_product_desc* d) {
+// Forward: the operands and the epilogue; 0 when all of it is sound.
+int check_forward(const wm_product_desc* d) {
+    const bool gated = d->act == WM_ACT_SWIGLU;
+    WM_CHECK_ARG(!gated || d->out % 2 == 0);
+    WM_CHECK_ARG(d->y_type == d->dtype || d->y_type == WM_F32);
+    WM_CHECK_ARG(al(d->x, 2) && al(d->w, 2) && al(d->bias, 2) && al(d->residual, 2) && al(d->pre, 2));
+    WM_CHECK_ARG(al(d->y, size_of(d->y_type)));
+    const int cols = gated ? d->out / 2 : d->out;
+    WM_CHECK_ARG(d->rows == 0 || d->ldy >= cols);
+    WM_CHECK_ARG(!d->residual || d->ld_residual >= cols);
+    WM_CHECK_ARG(!d->pre || d->ld_pre >= d->out);
+    return WM_OK;
+}
+int check_backward(const wm_product_desc* d) {
+    WM_CHECK_ARG(d->act == WM_ACT_NONE);
+    WM_CHECK_ARG(al(d->x, 2) && al(d->w, 2) && al(d->dz, 2));
+    WM_CHECK_ARG(d->rows == 0 || d->ld_dz >= d->out);
+    return WM_OK;
+}
+
+ProductArgs arguments(const wm_product_desc* d) {
     ProductArgs a = {};
     a.bf16 = d->dtype == WM_BF16;
     a.rows = d->rows;
@@ -51,32 +71,7 @@ ProductArgs common(const wm_product_desc* d) {
     a.ldx = d->ldx;
     a.w = (const uint16_t*)d->w;
     a.ldw = d->ldw;
-    a.w_stride = d->w_stride;
-    return a;
-}
-}  // namespace
-
-extern "C" int64_t wm_product_workspace_size(const wm_product_desc* d, int backward) {
-    (void)backward;
-    if (int rc = check_desc(d)) return rc;
-    return 0;
-}
-
-extern "C" int wm_product(const wm_product_desc* d, void* ws, int64_t ws_bytes, void* stream) {
-    (void)ws;
-    (void)ws_bytes;
-    if (int rc = check_desc(d)) return rc;
-    const bool gated = d->act == WM_ACT_SWIGLU;
-    WM_CHECK_ARG(!gated || d->out % 2 == 0);
-    const int cols = gated ? d->out / 2 : d->out;
-    WM_CHECK_ARG(d->y_type == d->dtype || d->y_type == WM_F32);
-    if (d->rows == 0) return WM_OK;
-    WM_CHECK_ARG(d->x && d->w && d->y);
-    WM_CHECK_ARG(al(d->x, 2) && al(d->w, 2) && al(d->bias, 2) && al(d->residual, 2) && al(d->pre, 2));
-    WM_CHECK_ARG(al(d->y, size_of(d->y_type)));
-    WM_CHECK_ARG(d->ldy >= cols && (!d->residual || d->ld_residual >= cols) && (!d->pre || d->ld_pre >= d->out));
-    if (wm_init()) return WM_ERR;
-    ProductArgs a = common(d);
+    a.w_stride = d->n_groups > 1 ? d->w_stride : 0;
     a.act = d->act;
     a.bias = (const uint16_t*)d->bias;
     a.res = (const uint16_t*)d->residual;
@@ -86,36 +81,51 @@ extern "C" int wm_product(const wm_product_desc* d, void* ws, int64_t ws_bytes, 
     a.y_f32 = d->y_type == WM_F32;
     a.pre = (uint16_t*)d->pre;
     a.ldpre = d->ld_pre;
-    WM_FAIL_HIP(launch_product(a, S(stream)));
+    a.dz = (const uint16_t*)d->dz;
+    a.lddz = d->ld_dz;
+    a.split = 1;
+    return a;
+}
+}  // namespace
+
+extern "C" int64_t wm_product_workspace_size(const wm_product_desc* d, int backward) {
+    if (int rc = check_desc(d)) return rc;
+    if (int rc = backward ? check_backward(d) : check_forward(d)) return rc;
+    return product_workspace(arguments(d), backward != 0);
+}
+
+extern "C" int wm_product(const wm_product_desc* d, void* ws, int64_t ws_bytes, void* stream) {
+    if (int rc = check_desc(d)) return rc;
+    if (int rc = check_forward(d)) return rc;
+    if (d->rows == 0) return WM_OK;
+    WM_CHECK_ARG(d->x && d->w && d->y);
+    const ProductArgs a = arguments(d);
+    const int64_t need = product_workspace(a, false);
+    WM_CHECK_ARG(need == 0 || (ws && al(ws, 256) && ws_bytes >= need));
+    if (wm_init()) return WM_ERR;
+    WM_FAIL_HIP(launch_product(a, (uint8_t*)ws, S(stream)));
     return WM_OK;
 }
 
-extern "C" int wm_product_backward(const wm_product_desc* d, const void* dz, int64_t ld_dz, void* dx, int64_t ld_dx,
-                                   void* dw, int dw_type, float* db, void* ws, int64_t ws_bytes, void* stream) {
-    (void)ws;
-    (void)ws_bytes;
+extern "C" int wm_product_backward(const wm_product_desc* d, void* dx, int64_t ld_dx, void* dw, int dw_type, float* db,
+                                   void* ws, int64_t ws_bytes, void* stream) {
     if (int rc = check_desc(d)) return rc;
-    WM_CHECK_ARG(d->act == WM_ACT_NONE);
+    if (int rc = check_backward(d)) return rc;
     WM_CHECK_ARG(!dw || dw_type == d->dtype || dw_type == WM_F32);
-    WM_CHECK_ARG(d->rows == 0 || (dz && al(dz, 2) && ld_dz >= d->out));
-    WM_CHECK_ARG(!dx || (al(dx, 2) && ld_dx >= d->in && d->w && al(d->w, 2)));
-    WM_CHECK_ARG((!dw && !db) || d->rows == 0 || (d->x && al(d->x, 2)));
+    WM_CHECK_ARG(d->rows == 0 || d->dz);
+    WM_CHECK_ARG(!dx || (al(dx, 2) && ld_dx >= d->in && d->w));
+    WM_CHECK_ARG((!dw && !db) || d->rows == 0 || d->x);
     WM_CHECK_ARG(al(dw, size_of(dw_type)) && al(db, 4));
+    ProductArgs a = arguments(d);
+    const int64_t need = product_workspace(a, true);
+    WM_CHECK_ARG(need == 0 || (ws && al(ws, 256) && ws_bytes >= need));
     if (wm_init()) return WM_ERR;
-    ProductArgs a = common(d);
-    a.dz = (const uint16_t*)dz;
-    a.lddz = ld_dz;
-    if (dx && d->rows) {
-        a.dx = (uint16_t*)dx;
-        a.lddx = ld_dx;
-        WM_FAIL_HIP(launch_product_dx(a, S(stream)));
-    }
-    if (dw || db) {
-        a.dw = dw;
-        a.dw_f32 = dw_type == WM_F32;
-        a.db = db;
-        WM_FAIL_HIP(launch_product_dw(a, S(stream)));
-    }
+    a.dx = (uint16_t*)dx;
+    a.lddx = ld_dx;
+    a.dw = dw;
+    a.dw_f32 = dw_type == WM_F32;
+    a.db = db;
+    WM_FAIL_HIP(launch_product_backward(a, (uint8_t*)ws, S(stream)));
     return WM_OK;
 }
 

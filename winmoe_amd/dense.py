@@ -32,7 +32,7 @@ _TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _li
 
 # wm_product_desc as a byte string: filling a ctypes structure field by field
 # takes 3 us of a call whose kernel may take 5.
-_DESC = struct.Struct("8i14q")
+_DESC = struct.Struct("8i16q")
 
 
 # Checks cost the host a few microseconds a call, so they are plain Python on
@@ -170,7 +170,7 @@ def _product(x, w, offsets, token, bias, act, residual, out, pre, out_dtype, str
     if pre is not None:
         pp, ldp = pre.data_ptr(), _rows(pre, rows, outs, dt, "pre")
     desc = _DESC.pack(_TYPES[dt], rows, inn, outs, E, x_rows, a, _TYPES[yt], off, tok, xp, ldx, wp, ldw, stride, bp,
-                      rp, ldr, out.data_ptr(), ldy, pp, ldp)
+                      rp, ldr, out.data_ptr(), ldy, pp, ldp, 0, 0)
     L = load()
     ws, nb = _workspace(L, desc, 0, x, stream)
     check(L.wm_product(desc, ws.data_ptr() if nb else None, nb, _raw(stream, x)), "wm_product")
@@ -196,11 +196,11 @@ def _product_backward(dz, x, w, offsets, token, need_dx, need_dw, need_db, dw_dt
             db = _new(x, w.shape[:-1], torch.float32, stream)
         dbp = _dense(db, w.shape[:-1], torch.float32, "db")
     desc = _DESC.pack(_TYPES[dt], rows, inn, outs, E, x_rows, 0, _TYPES[dt], off, tok, xp, ldx, wp, ldw, stride,
-                      0, 0, 0, 0, 0, 0, 0)
+                      0, 0, 0, 0, 0, 0, 0, dz.data_ptr(), ldz)
     L = load()
     ws, nb = _workspace(L, desc, 1, x, stream)
-    check(L.wm_product_backward(desc, dz.data_ptr(), ldz, dxp, lddx, dwp, _TYPES[wt], dbp,
-                                ws.data_ptr() if nb else None, nb, _raw(stream, x)), "wm_product_backward")
+    check(L.wm_product_backward(desc, dxp, lddx, dwp, _TYPES[wt], dbp, ws.data_ptr() if nb else None, nb,
+                                _raw(stream, x)), "wm_product_backward")
     return dx, dw, db
 
 
