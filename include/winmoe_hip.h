@@ -325,6 +325,13 @@ typedef struct wm_product_desc {
  * calls. */
 int64_t wm_product_workspace_size(const wm_product_desc* d, int backward);
 
+/* Which kernel a product runs on (a property of sizes, types and alignment, for
+ * tests and profiles): direction 0 forward, 1 dx, 2 dw.  Returns an index of
+ * WM_PRODUCT_KERNELS, or < 0 for a bad descriptor; *parts is the number of
+ * workgroups that share an output tile's contraction. */
+#define WM_PRODUCT_KERNELS "any128", "any32", "few", "256x256", "128x128", "128x64", "128x32", "64x64", "64x32", "64x16"
+int wm_product_plan(const wm_product_desc* d, int direction, int* parts);
+
 /* y[r] = act(W_e x[token[r]] + bias_e) + residual[r] for every row r of every
  * group e. */
 int wm_product(const wm_product_desc* d, void* ws, int64_t ws_bytes, void* stream);

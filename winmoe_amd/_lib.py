@@ -33,6 +33,7 @@ FLAG_SPIN_PROBE = 16
 FLAG_PREFILL_PASS16 = 32
 FLAG_PREFILL_PASS32 = 64
 
+PRODUCT_KERNELS = ("any128", "any32", "few", "256x256", "128x128", "128x64", "128x32", "64x64", "64x32", "64x16")
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "swiglu": 4}
 
 _vp, _i64 = C.c_void_p, C.c_int64
@@ -112,6 +113,7 @@ SIGNATURES = {
                                 _vp]),
     "wm_expert_workspace_size": (_i64, [C.c_int, C.c_int]),
     "wm_product_workspace_size": (_i64, [_vp, C.c_int]),
+    "wm_product_plan": (C.c_int, [_vp, C.c_int, C.POINTER(C.c_int)]),
     "wm_product": (C.c_int, [_vp, _vp, _i64, _vp]),
     "wm_product_backward": (C.c_int, [_vp, _vp, _i64, _vp, C.c_int, _vp, _vp, _i64, _vp]),
     "wm_act_backward": (C.c_int, [C.c_int, C.c_int, _i64, C.c_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),

@@ -51,6 +51,8 @@ struct ProductArgs {
 
 // Bytes of workspace that a direction (backward: DX and DW together) uses.
 int64_t product_workspace(const ProductArgs& a, bool backward);
+// The kernel of a direction (index of WM_PRODUCT_KERNELS) and its parts.
+int product_plan(const ProductArgs& a, int dir, int* parts);
 // ws holds product_workspace() bytes, 256-byte aligned.
 int launch_product(const ProductArgs& a, uint8_t* ws, hipStream_t s);
 int launch_product_backward(const ProductArgs& a, uint8_t* ws, hipStream_t s);     // dx, dw, db: those not NULL

@@ -41,21 +41,6 @@ template <bool BF> WM_DEV f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// 8 values at p, of which the first n exist; the others are zero.  p needs no
-// alignment beyond its type's.
-WM_DEV uint4 load8(const uint16_t* p, int n) {
-    uint4 v = {0, 0, 0, 0};
-    if (n >= 8) {
-        __builtin_memcpy(&v, p, 16);
-    } else {
-        uint16_t e[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) e[i] = i < n ? p[i] : 0;
-        __builtin_memcpy(&v, e, 16);
-    }
-    return v;
-}
-
 // Workgroup's group: `qt` counts the tiles of BQ rows over all groups.
 // Offsets are clamped to [0, rows], so whatever they hold no row outside is
 // touched.  Every wave looks it up by itself.
@@ -870,7 +855,7 @@ struct TileCost {
     float alone, share;
 };
 static constexpr TileCost kTiles[] = {
-    {T256, 256, 256, 1, 1.40f, 1.65f}, {T128, 128, 128, 2, 0.70f, 0.54f},  {T128x64, 128, 64, 2, 0.58f, 0.36f},
+    {T256, 256, 256, 1, 1.40f, 1.65f}, {T128, 128, 128, 2, 0.82f, 0.54f},  {T128x64, 128, 64, 2, 0.58f, 0.36f},
     {T128x32, 128, 32, 2, 0.46f, 0.33f}, {T64, 64, 64, 2, 0.40f, 0.27f},   {T64x32, 64, 32, 3, 0.34f, 0.20f},
     {T64x16, 64, 16, 4, 0.34f, 0.15f},
 };
@@ -891,15 +876,17 @@ static int64_t row_tiles(const ProductArgs& a, int bq) {
 
 // The tile and the number of parts with the least estimated time.  The chip is
 // taken as 256 CUs; the rows of a group are taken as even, as the host does not
-// know them.  A split pays a second kernel and the parts' way to memory and
-// back: 3 us and 3 TB/s.
+// know them.  Reading the weights (writing, for dW) overlaps the products, but
+// not fully; tiles 64 wide read them in shorter rows.  A split pays a second
+// kernel (which has to look groups up) and the parts' way to memory and back:
+// 4 or 7 us and 2.5 TB/s.
 static Plan plan_tiles(const ProductArgs& a, int dir) {
     const double groups = a.offsets ? std::max(1.0, std::min((double)a.E, (double)a.rows)) : 1.0, per = a.rows / groups;
     const int outs = columns(a, dir);
     const bool gated = dir == FWD && a.act == WM_ACT_SWIGLU;
     const double steps = dir == FWD ? a.in : dir == DX ? a.out : per;
     const double stages = std::max(1.0, std::ceil(steps / BK));
-    const double memory = groups * a.in * a.out * 2.0 * (dir == DW ? 1 + a.dw_f32 : 1) / 5.6e6;     // us
+    const double memory = (dir == DW ? a.E * (1.0 + a.dw_f32) : groups) * a.in * a.out * 2.0 / 5.6e6;       // us
     const double sums = (dir == DW ? (double)a.E * a.out * a.in : (double)a.rows * (dir == FWD ? a.out : a.in)) * 8.0;
     Plan best{T128, 1};
     double least = 1e30;
@@ -911,7 +898,8 @@ static Plan plan_tiles(const ProductArgs& a, int dir) {
             if (s > 1 && s * sums > 512e6) break;
             const double n = std::max(1.0, p * q * s / 256), turns = std::max(1.0, n / t.resident);
             const double work = std::ceil(stages / s) * std::max(t.alone * turns, t.share * n) + 2.0 * turns;
-            const double us = std::max(work, t.bp < 128 ? 1.15 * memory : memory) + (s > 1 ? 3.0 + s * sums / 3e6 : 0.0);
+            const double stream = t.bp < 128 ? 1.15 * memory : memory;
+            const double us = std::max(work, stream) + 0.3 * std::min(work, stream) + (s > 1 ? (a.offsets ? 7.0 : 4.0) + s * sums / 2.5e6 : 0.0);
             if (us < least) {
                 least = us;
                 best = {t.k, s};
@@ -976,6 +964,12 @@ static ProductArgs without_dx(const ProductArgs& a) {
     ProductArgs b = a;
     if (!b.dw) b.in = 1;
     return b;
+}
+
+int product_plan(const ProductArgs& a, int dir, int* parts) {
+    const Plan p = dir == DW ? plan_tiles(a, DW) : plan_rows(a, dir);
+    *parts = p.split;
+    return p.k;
 }
 
 int64_t product_workspace(const ProductArgs& a, bool backward) {

@@ -94,6 +94,13 @@ extern "C" int64_t wm_product_workspace_size(const wm_product_desc* d, int backw
     return product_workspace(arguments(d), backward != 0);
 }
 
+extern "C" int wm_product_plan(const wm_product_desc* d, int direction, int* parts) {
+    if (int rc = check_desc(d)) return rc;
+    WM_CHECK_ARG(direction >= FWD && direction <= DW && parts && d->rows > 0);
+    if (int rc = direction == FWD ? check_forward(d) : check_backward(d)) return rc;
+    return product_plan(arguments(d), direction, parts);
+}
+
 extern "C" int wm_product(const wm_product_desc* d, void* ws, int64_t ws_bytes, void* stream) {
     if (int rc = check_desc(d)) return rc;
     if (int rc = check_forward(d)) return rc;
