@@ -289,6 +289,7 @@ int64_t wm_expert_workspace_size(int H, int I);
 #define WM_ACT_SILU 2
 #define WM_ACT_GELU 3    /* z * Phi(z), exact */
 #define WM_ACT_SWIGLU 4  /* silu(gate) * up; W holds the gate rows, then the up rows */
+#define WM_ACT_SIGMOID 5
 typedef struct wm_product_desc {
     int32_t dtype;           /* WM_F16 or WM_BF16: x, w, bias, residual, pre, dz, dx */
     int32_t rows;            /* rows of the product (0: nothing to do) */

@@ -13,7 +13,7 @@ import math
 import torch
 
 TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}
-SLOPE = {"none": 1.0, "relu": 1.0, "silu": 1.1, "gelu": 1.13}
+SLOPE = {"none": 1.0, "relu": 1.0, "silu": 1.1, "gelu": 1.13, "sigmoid": 0.25}
 
 
 def rounding(v, dtype):
@@ -25,6 +25,8 @@ def act(z, name):
     if name == "swiglu":
         g, u = z.chunk(2, 1)
         return g * torch.sigmoid(g) * u
+    if name == "sigmoid":
+        return torch.sigmoid(z)
     if name == "silu":
         return z * torch.sigmoid(z)
     if name == "gelu":

@@ -30,7 +30,7 @@ def desc(**kw):
 BAD = [dict(dtype=0), dict(dtype=8), dict(rows=-1), dict(rows=(1 << 30) + 1), dict(inn=0), dict(out=0),
        dict(inn=(1 << 26) + 1), dict(n_groups=0), dict(n_groups=2), dict(n_groups=(1 << 16) + 1, offsets=64),
        dict(offsets=66), dict(token=65), dict(x_rows=3), dict(x_rows=-1, token=64), dict(ldx=7), dict(ldw=7),
-       dict(n_groups=2, offsets=64, w_stride=127), dict(act=-1), dict(act=5), dict(x=None), dict(w=None), dict(y=None),
+       dict(n_groups=2, offsets=64, w_stride=127), dict(act=-1), dict(act=6), dict(x=None), dict(w=None), dict(y=None),
        dict(x=4097), dict(w=8193), dict(y=16385), dict(y_type=1), dict(y_type=0, y=16386), dict(ldy=15),
        dict(bias=65), dict(residual=65, ld_residual=16), dict(residual=64, ld_residual=15), dict(pre=64, ld_pre=15),
        dict(pre=65, ld_pre=16), dict(act=4, out=15), dict(act=4, ldy=7)]

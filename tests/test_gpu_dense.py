@@ -47,7 +47,7 @@ def test_linear(dense, size, dt):
     ref.within(dense.linear(x, w, out_dtype=F32), y, by, "fp32")
 
 
-@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "swiglu"])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "swiglu", "sigmoid"])
 @pytest.mark.parametrize("size", [(1, 256, 64), (5, 96, 34), (40, 1000, 130), (200, 128, 258), (300, 576, 512)], ids=str)
 def test_linear_epilogue(dense, size, act):
     """Bias, activation, residual, pre-activation, output in place of the residual, strided rows."""
@@ -386,7 +386,7 @@ def test_combine_backward(dense, size, dt):
 
 
 @pytest.mark.parametrize("dt", DT, ids=["bf16", "fp16"])
-@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "swiglu"])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "swiglu", "sigmoid"])
 @pytest.mark.parametrize("size", [(1, 8), (3, 5), (23, 4096), (70, 1001)], ids=str)
 def test_act_backward(dense, size, act, dt):
     """Bound: sums of two terms of at most 1.2 |dy| (|u|), each good to 16 steps of fp32."""

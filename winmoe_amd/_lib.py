@@ -34,7 +34,7 @@ FLAG_PREFILL_PASS16 = 32
 FLAG_PREFILL_PASS32 = 64
 
 PRODUCT_KERNELS = ("any128", "any32", "few", "256x256", "128x128", "128x64", "128x32", "64x64", "64x32", "64x16")
-ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "swiglu": 4}
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "swiglu": 4, "sigmoid": 5}
 
 _vp, _i64 = C.c_void_p, C.c_int64
 

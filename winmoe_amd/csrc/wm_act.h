@@ -58,6 +58,7 @@ WM_DEV float act_value(int act, float z, float u) {
         return z * cdf;
     }
     case WM_ACT_SWIGLU: return z * sigmoid(z) * u;
+    case WM_ACT_SIGMOID: return sigmoid(z);
     default: return z;
     }
 }
@@ -75,6 +76,10 @@ WM_DEV float act_slope(int act, float z) {
     case WM_ACT_SWIGLU: {
         const float s = sigmoid(z);
         return s * (1.0f + z * (1.0f - s));
+    }
+    case WM_ACT_SIGMOID: {
+        const float s = sigmoid(z);
+        return s * (1.0f - s);
     }
     default: return 1.0f;
     }

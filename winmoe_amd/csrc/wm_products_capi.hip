@@ -33,7 +33,7 @@ int check_desc(const wm_product_desc* d) {
     WM_CHECK_ARG(d->token || d->x_rows >= d->rows);
     WM_CHECK_ARG(d->ldx >= d->in && d->ldw >= d->in);
     WM_CHECK_ARG(d->n_groups == 1 || d->w_stride >= (int64_t)(d->out - 1) * d->ldw + d->in);
-    WM_CHECK_ARG(d->act >= WM_ACT_NONE && d->act <= WM_ACT_SWIGLU);
+    WM_CHECK_ARG(d->act >= WM_ACT_NONE && d->act <= WM_ACT_SIGMOID);
     return WM_OK;
 }
 
@@ -139,7 +139,7 @@ extern "C" int wm_product_backward(const wm_product_desc* d, void* dx, int64_t l
 extern "C" int wm_act_backward(int dtype, int act, int64_t rows, int cols, const void* dy, int64_t ld_dy,
                                const void* pre, int64_t ld_pre, void* dz, int64_t ld_dz, void* stream) {
     WM_CHECK_ARG(dtype_ok(dtype));
-    WM_CHECK_ARG(act >= WM_ACT_NONE && act <= WM_ACT_SWIGLU);
+    WM_CHECK_ARG(act >= WM_ACT_NONE && act <= WM_ACT_SIGMOID);
     WM_CHECK_ARG(rows >= 0 && rows <= kMaxRows && cols >= 1 && cols <= kMaxDim);
     if (rows == 0) return WM_OK;
     const int64_t wide = act == WM_ACT_SWIGLU ? 2 * (int64_t)cols : cols;

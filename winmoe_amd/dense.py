@@ -209,8 +209,9 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
            pre: Optional[torch.Tensor] = None, out_dtype=None, stream=None) -> torch.Tensor:
     """act(x W^T + bias) + residual: x [T][in], W [out][in], bias [out], residual [T][columns].
 
-    act is "none", "relu", "silu", "gelu" (exact) or "swiglu": silu(gate) * up
-    with the gate rows of W before the up rows, the result half as wide.  x, W,
+    act is "none", "relu", "silu", "gelu" (exact), "sigmoid" or "swiglu":
+    silu(gate) * up with the gate rows of W before the up rows, the result half
+    as wide.  x, W,
     bias and residual are of one 16-bit type; the result is of that type or
     float32 (out_dtype, or out's).  pre [T][out] receives x W^T + bias for the
     way back.  residual may be out itself; no other output may overlap an input."""
@@ -346,3 +347,122 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, row: torch.Tensor, w: 
                                           rp, wp, T, K, H, dyp, lddy, dwp, _raw(stream, y)),
           "wm_combine_rows_backward")
     return dy, dw
+
+
+# ------------------------------------------------------------------ layer
+
+class Gradients(NamedTuple):
+    """What ``FloatMoELayer.backward`` returns; None for parts the layer does not have."""
+    x: torch.Tensor                         # [T][H]
+    w: torch.Tensor                         # routing weights, float32 [T][K]
+    gate_up: torch.Tensor                   # [E][2 I][H]
+    down: torch.Tensor                      # [E][H][I]
+    shared_gate_up: Optional[torch.Tensor]  # [2 I_s][H]
+    shared_down: Optional[torch.Tensor]     # [H][I_s]
+    shared_gate: Optional[torch.Tensor]     # [1][H]
+
+
+class FloatMoELayer:
+    """A mixture-of-experts layer whose weights are fp16 or bf16, for any number of tokens.
+
+    gate_up [E][2 I][H] holds each expert's gate rows, then its up rows; down
+    is [E][H][I].  The optional shared expert has the same form without E, and
+    an optional gate [1][H] (its output counts sigmoid(x . gate) times).  The
+    mathematics is ``MoELayer``'s (winmoe_inference.c:1684-2027), which takes
+    the quantised formats; here every product runs on 16-bit values with fp32
+    sums, and the layer can be trained: ``forward(..., keep=True)`` hands out
+    what ``backward`` needs."""
+
+    def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, K: int, router: Optional[torch.Tensor] = None,
+                 shared_gate_up: Optional[torch.Tensor] = None, shared_down: Optional[torch.Tensor] = None,
+                 shared_gate: Optional[torch.Tensor] = None):
+        dt = _dtype16(gate_up, "gate_up")
+        if gate_up.dim() != 3 or gate_up.shape[1] % 2:
+            raise ValueError(f"gate_up must be [E][2 I][H], got {list(gate_up.shape)}")
+        self.E, self.I, self.H, self.K, self.dtype = gate_up.shape[0], gate_up.shape[1] // 2, gate_up.shape[2], K, dt
+        if not 1 <= K <= self.E:
+            raise ValueError(f"K must lie in [1, {self.E}], got {K}")
+        _dense(gate_up, gate_up.shape, dt, "gate_up")
+        _dense(down, (self.E, self.H, self.I), dt, "down")
+        if router is not None:
+            _dense(router, (self.E, self.H), torch.float32, "router")
+        if (shared_gate_up is None) != (shared_down is None) or (shared_gate is not None and shared_down is None):
+            raise ValueError("a shared expert needs shared_gate_up and shared_down")
+        if shared_down is not None:
+            _dense(shared_down, (self.H, shared_down.shape[-1]), dt, "shared_down")
+            _dense(shared_gate_up, (2 * shared_down.shape[1], self.H), dt, "shared_gate_up")
+        if shared_gate is not None:
+            _dense(shared_gate, (1, self.H), dt, "shared_gate")
+        self.gate_up, self.down, self.router = gate_up, down, router
+        self.shared_gate_up, self.shared_down, self.shared_gate = shared_gate_up, shared_down, shared_gate
+
+    def route(self, x: torch.Tensor):
+        """(ids int32 [T][K], weights float32 [T][K]) by the layer's router, one token after another (``router_topk``)."""
+        from .moe import router_topk
+        if self.router is None:
+            raise ValueError("the layer has no router")
+        _rows(x, x.shape[0], self.H, self.dtype, "x")
+        ids = x.new_empty((x.shape[0], self.K), dtype=torch.int32)
+        w = x.new_empty((x.shape[0], self.K), dtype=torch.float32)
+        for t, h in enumerate(x.float()):
+            ids[t], w[t] = router_topk(h, self.router, self.K)
+        return ids, w
+
+    def forward(self, x: torch.Tensor, ids: torch.Tensor, w: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                keep: bool = False):
+        """The layer's output [T][H] for x [T][H], picks ids int32 [T][K] and weights w float32 [T][K].
+
+        A pick outside [0, E) counts as nothing.  residual [T][H] (x's type or
+        float32) is added, and the result is of its type, else of x's.  With
+        keep, returns (output, what ``backward`` takes)."""
+        T, K = x.shape[0], self.K
+        _rows(x, T, self.H, self.dtype, "x")
+        _dense(ids, (T, K), torch.int32, "ids")
+        _dense(w, (T, K), torch.float32, "w")
+        R = T * K
+        g = group_by_expert(ids, self.E)
+        shared = self.shared_down is not None
+        pre = x.new_empty((R, 2 * self.I)) if keep else None
+        h = grouped_matmul(x, self.gate_up, g.offsets, token=g.token, act="swiglu", pre=pre)
+        # the shared expert's rows stand behind the routed ones: one more pick of every token
+        y = x.new_empty((R + T if shared else R, self.H))
+        grouped_matmul(h, self.down, g.offsets, out=y[:R])
+        row, weight, pre_s, hs = g.row, w, None, None
+        if shared:
+            pre_s = x.new_empty((T, self.shared_gate_up.shape[0])) if keep else None
+            hs = linear(x, self.shared_gate_up, act="swiglu", pre=pre_s)
+            linear(hs, self.shared_down, out=y[R:])
+            s = (linear(x, self.shared_gate, act="sigmoid", out_dtype=torch.float32) if self.shared_gate is not None
+                 else w.new_ones((T, 1)))
+            last = torch.arange(R, R + T, dtype=torch.int32, device=x.device).view(T, 1)
+            row, weight = torch.cat([g.row, last], 1), torch.cat([w, s], 1)
+        out = combine(y, row, weight, residual=residual)
+        return (out, (x, g, pre, h, y, row, weight, pre_s, hs)) if keep else out
+
+    def backward(self, dout: torch.Tensor, kept, dw_dtype=None) -> Gradients:
+        """Gradients given dout [T][H] (x's type or float32) and what ``forward(..., keep=True)`` handed out.
+
+        The matrices' gradients are of the layer's type or float32 (dw_dtype);
+        the residual's gradient is dout itself."""
+        x, g, pre, h, y, row, weight, pre_s, hs = kept
+        T, K, R = x.shape[0], self.K, x.shape[0] * self.K
+        dy, dweight = combine_backward(dout, y, row, weight)
+        dh, ddown, _ = grouped_matmul_backward(dy[:R], h, self.down, g.offsets, dw_dtype=dw_dtype)
+        dz = act_backward(dh, pre, "swiglu")
+        # one buffer for the parts of dx, which are summed and rounded once
+        extra = 0 if hs is None else 1 if self.shared_gate is None else 2       # rows per token that the shared expert adds
+        parts = x.new_empty((R + extra * T, self.H))
+        _, dgu, _ = grouped_matmul_backward(dz, x, self.gate_up, g.offsets, token=g.token, dw_dtype=dw_dtype, dx=parts[:R])
+        dsgu = dsd = dsg = None
+        rows = [g.row]
+        if hs is not None:
+            dhs, dsd, _ = linear_backward(dy[R:], hs, self.shared_down, dw_dtype=dw_dtype)
+            dzs = act_backward(dhs, pre_s, "swiglu")
+            _, dsgu, _ = linear_backward(dzs, x, self.shared_gate_up, dw_dtype=dw_dtype, dx=parts[R:R + T])
+            if self.shared_gate is not None:
+                s = weight[:, K:]
+                ds = (dweight[:, K:] * s * (1.0 - s)).to(self.dtype)
+                _, dsg, _ = linear_backward(ds, x, self.shared_gate, dw_dtype=dw_dtype, dx=parts[R + T:])
+            rows.append(torch.arange(R, parts.shape[0], dtype=torch.int32, device=x.device).view(extra, T).T)
+        dx = combine(parts, torch.cat(rows, 1) if len(rows) > 1 else g.row)
+        return Gradients(dx, dweight[:, :K], dgu, ddown, dsgu, dsd, dsg)

@@ -308,8 +308,8 @@ def expert_slice(g: GGUFFile, name: str, e: int) -> np.ndarray:
 
 
 def _router_fp32(g: "GGUFFile", name: str, t, E: int, H: int, device) -> torch.Tensor:
-    """The router as fp32 [E][H] on the device.  F32 is taken as is; F16 is
-    widened exactly; quantised routers (Q8_0, Q2_K .. Q6_K) are dequantised
+    """The router as fp32 [E][H] on the device.  F32 is taken as is; F16 and
+    BF16 are widened exactly; quantised routers (Q8_0, Q2_K .. Q6_K) are dequantised
     exactly by the library.  The reference dispatches a quantised router
     through quant_matvec (transformer.h:120-123), whose Q8_0 / K-quant paths
     round the activations to int8 first, so its logits for such a router can
@@ -322,12 +322,48 @@ def _router_fp32(g: "GGUFFile", name: str, t, E: int, H: int, device) -> torch.T
         w = torch.from_numpy(raw.view(np.float32)).to(device)
     elif t.ggml_type == 1:
         w = torch.from_numpy(raw.view(np.float16).astype(np.float32)).to(device)
+    elif t.ggml_type == _lib.BF16:
+        w = torch.from_numpy((raw.view(np.uint16).astype(np.uint32) << 16).view(np.float32)).to(device)
     elif t.ggml_type in _lib.QUANT_TYPES:
         from .moe import dequantize
         w = dequantize(torch.from_numpy(raw).to(device), t.ggml_type)
     else:
-        raise GGUFError(f"router type {t.ggml_type} is not supported (F32, F16, Q8_0, Q2_K .. Q6_K are)")
+        raise GGUFError(f"router type {t.ggml_type} is not supported (F32, F16, BF16, Q8_0, Q2_K .. Q6_K are)")
     return w.view(E, H).contiguous()
+
+
+def _float_layer(g: "GGUFFile", pre: str, ggml_type: int, dims, K: int, router, device):
+    """Layer of F16 or BF16 tensors: a FloatMoELayer with gate and up stacked per expert."""
+    import torch
+
+    from .dense import FloatMoELayer
+    H, I, E = dims
+    dt = torch.float16 if ggml_type == 1 else torch.bfloat16
+
+    def dev(n, *shape):
+        t = g.find(pre + n)
+        if t is None:
+            raise GGUFError(f"missing tensor {pre + n}")
+        if t.ggml_type != ggml_type or t.dims != tuple(reversed(shape)):
+            raise GGUFError(f"{pre + n} is {t.dims} of type {t.ggml_type}, expected {tuple(reversed(shape))} of type {ggml_type}")
+        raw = np.array(g.data(pre + n), copy=True)
+        return torch.from_numpy(raw.view(np.int16)).view(dt).view(*shape).to(device)
+
+    def gate_up(kind, *shape):
+        return torch.cat([dev(f"ffn_gate_{kind}.weight", *shape), dev(f"ffn_up_{kind}.weight", *shape)], len(shape) - 2).contiguous()
+
+    shared = {}
+    ts = g.find(pre + "ffn_gate_shexp.weight")
+    if ts is not None:
+        Is = ts.dims[1]
+        shared = {"shared_gate_up": gate_up("shexp", Is, H), "shared_down": dev("ffn_down_shexp.weight", H, Is)}
+        tgi = g.find(pre + "ffn_gate_inp_shexp.weight")
+        if tgi is not None:
+            if tgi.ggml_type != 0 or tgi.dims != (H,):
+                raise GGUFError(f"shared-expert gate must be F32 [{H}]")
+            gi = torch.from_numpy(np.array(g.data(pre + "ffn_gate_inp_shexp.weight"), copy=True).view(np.float32))
+            shared["shared_gate"] = gi.view(1, H).to(device).to(dt)
+    return FloatMoELayer(gate_up("exps", E, I, H), dev("ffn_down_exps.weight", E, H, I), K, router=router, **shared)
 
 
 def moe_layer_from_gguf(g: GGUFFile, layer: int, K: Optional[int] = None, device="cuda", max_tokens: int = 256,
@@ -339,7 +375,12 @@ def moe_layer_from_gguf(g: GGUFFile, layer: int, K: Optional[int] = None, device
     ``blk.L.ffn_down_exps.weight`` [I, H, E] in one quantised type each;
     optional shared expert ``blk.L.ffn_{gate,up,down}_shexp.weight`` and its
     fp32 gate ``blk.L.ffn_gate_inp_shexp.weight`` [H].  K defaults to the
-    model's ``<arch>.expert_used_count``."""
+    model's ``<arch>.expert_used_count``.
+
+    Experts of type F16 or BF16 (gate, up, down and shared alike) make a
+    ``dense.FloatMoELayer`` instead, which takes any number of tokens and has
+    no workspace: max_tokens and multi_kernel do not apply to it.  The shared
+    expert's gate is then rounded to that type."""
     import torch
 
     from . import _lib
@@ -363,9 +404,10 @@ def moe_layer_from_gguf(g: GGUFFile, layer: int, K: Optional[int] = None, device
     if td.dims != (I, H, E):
         raise GGUFError(f"down experts are {td.dims}, expected {(I, H, E)}")
     types = (tg.ggml_type, tu.ggml_type, td.ggml_type)
+    floats = types[0] in (_lib.F16, _lib.BF16) and types == (types[0],) * 3
     for t in types:
-        if t not in _lib.QUANT_TYPES:
-            raise GGUFError(f"expert type {t} is not supported (Q8_0, Q2_K .. Q6_K are)")
+        if not floats and t not in _lib.QUANT_TYPES:
+            raise GGUFError(f"expert type {t} is not supported (Q8_0, Q2_K .. Q6_K are; F16 and BF16 for all three)")
     if K is None:
         K = int(g.kv.get(f"{g.arch()}.expert_used_count", 0))
         if K <= 0:
@@ -376,6 +418,8 @@ def moe_layer_from_gguf(g: GGUFFile, layer: int, K: Optional[int] = None, device
         if tr.dims != (H, E):
             raise GGUFError(f"router must be [{H}, {E}], got {tr.dims}")
         router = _router_fp32(g, pre + "ffn_gate_inp.weight", tr, E, H, device)
+    if floats:
+        return _float_layer(g, pre, types[0], tg.dims, K, router, device)
     shared = None
     if g.find(pre + "ffn_gate_shexp.weight") is not None:
         sg, su, sd = need("ffn_gate_shexp.weight"), need("ffn_up_shexp.weight"), need("ffn_down_shexp.weight")
