@@ -81,3 +81,40 @@ def grouping(ids, E):
         offsets.append(len(token))
     token += [-1] * (T * K - len(token))
     return torch.tensor(offsets, dtype=torch.int32), torch.tensor(token, dtype=torch.int32), row
+
+
+# Shapes (rows, in, out, groups) that between them run every kernel of the
+# products, whole and in parts, plain and grouped: test_dense_host.py checks
+# that they still do.  Ragged in every dimension where the kernel allows it.
+KERNEL_SHAPES = {
+    "forward": [(1, 72, 40, 1), (3000, 200, 4104, 1), (4000, 264, 2056, 9), (4000, 136, 1032, 1), (4000, 72, 1032, 3),
+                (130, 200, 8200, 3), (17, 2056, 8200, 1), (16, 2056, 520, 9), (4000, 136, 520, 1), (4000, 136, 520, 3),
+                (3000, 4104, 136, 1), (3000, 4104, 136, 3), (16, 136, 4104, 9), (16, 2056, 264, 9), (19, 136, 24, 1),
+                (5, 136, 24, 3), (17, 1032, 16, 1), (2, 2056, 24, 3), (2000, 136, 520, 1), (4000, 136, 264, 3),
+                (1000, 2056, 16, 1), (1000, 2056, 24, 3), (200, 71, 56, 3), (50, 71, 56, 3), (5, 71, 57, 3), (700, 71, 57, 1),
+                (3, 2056, 2056, 3), (1000, 136, 8200, 9), (2000, 2056, 24, 3)],
+    "dx": [(3000, 2056, 72, 1), (4000, 1032, 136, 9), (4000, 2056, 200, 9), (3000, 4104, 136, 1), (2000, 520, 8200, 1),
+           (2000, 520, 8200, 3), (260, 4104, 72, 9), (3, 2056, 8200, 1), (130, 264, 4104, 9), (4000, 520, 72, 1),
+           (4000, 520, 72, 3), (3000, 136, 4104, 1), (2000, 72, 8200, 9), (16, 4104, 72, 9), (1, 2056, 2056, 1),
+           (16, 264, 2056, 9), (5, 72, 24, 1), (5, 72, 24, 3), (3, 72, 1032, 1), (3, 72, 2056, 3), (2000, 520, 72, 1),
+           (2000, 520, 72, 3), (1000, 72, 2056, 1), (1000, 72, 2056, 3), (50, 71, 57, 3), (700, 71, 57, 1),
+           (130, 200, 4104, 9), (3000, 4104, 136, 3)],
+    "dw": [(200, 4104, 520, 1), (300, 4104, 24, 9), (4000, 72, 8200, 1), (130, 2056, 8200, 1), (700, 1032, 1032, 9),
+           (70, 72, 24, 1), (70, 72, 24, 3), (1000, 72, 24, 1), (4000, 72, 24, 3), (1000, 71, 57, 1), (130, 264, 8200, 1)],
+}
+
+
+def plan(lib, rows, inn, out, groups, direction, parts):
+    """The kernel a product of contiguous bf16 operands runs on (wm_product_plan)."""
+    import ctypes as C
+
+    from winmoe_amd import _lib
+    d = _lib.ProductDesc()
+    d.dtype, d.rows, d.inn, d.out, d.n_groups, d.x_rows, d.y_type = _lib.BF16, rows, inn, out, groups, rows, _lib.BF16
+    d.x, d.w, d.y, d.dz, d.offsets = 4096, 4096, 4096, 4096, 4096 if groups > 1 else None
+    d.ldx, d.ldw, d.w_stride, d.ldy, d.ld_dz = inn, inn, inn * out, out, out
+    p = C.c_int()
+    k = lib.wm_product_plan(C.byref(d), direction, C.byref(p))
+    assert k >= 0
+    parts.append(p.value)
+    return _lib.PRODUCT_KERNELS[k]

@@ -6,7 +6,7 @@ import ctypes as C
 import pytest
 import torch
 
-from dense_ref import grouping
+from dense_ref import KERNEL_SHAPES, grouping, plan
 
 
 @pytest.fixture(scope="module")
@@ -127,3 +127,41 @@ def test_reference_grouping():
     off, token, row = grouping(torch.tensor([[2, 0], [-1, 2], [0, 3]]), 3)
     assert off.tolist() == [0, 2, 2, 4] and token.tolist() == [0, 2, 0, 1, -1, -1]
     assert row.tolist() == [[2, 0], [-1, 3], [1, -1]]
+
+
+def test_kernel_shapes_run_every_kernel(lib):
+    """The shapes of the GPU tests reach every kernel, whole and in parts, plain and grouped, that any of a wide
+    range of shapes reaches; wm_product_plan knows the same names as the Python binding."""
+    import itertools
+    import re
+
+    from winmoe_amd import _lib
+    header = open(_lib.os.path.join(_lib.PKG, "..", "include", "winmoe_hip.h")).read()
+    names = re.search(r"#define WM_PRODUCT_KERNELS (.*)", header).group(1)
+    assert tuple(re.findall(r'"(\w+)"', names)) == _lib.PRODUCT_KERNELS
+    reach, have = set(), set()
+    for i, direction in enumerate(("forward", "dx", "dw")):
+        for rows, inn, out, groups in KERNEL_SHAPES[direction]:
+            p = []
+            have.add((direction, plan(lib, rows, inn, out, groups, i, p), p[0] > 1, groups > 1))
+        for rows, inn, out, groups in itertools.product((1, 3, 16, 17, 50, 130, 700, 2000, 4000), (64, 71, 264, 1032, 4096),
+                                                        (16, 57, 136, 520, 2056, 8200), (1, 3, 9, 64)):
+            p = []
+            reach.add((direction, plan(lib, rows, inn, out, groups, i, p), p[0] > 1, groups > 1))
+    assert not reach - have, sorted(reach - have)
+
+
+def test_workspace_is_asked_for_and_checked(lib):
+    """A call whose size query is not 0 refuses a missing, short or unaligned workspace."""
+    d = desc(rows=1000, x_rows=1000, inn=2056, out=16, ldx=2056, ldw=2056)          # in parts
+    need = lib.wm_product_workspace_size(C.byref(d), 0)
+    assert need >= 2 * 1000 * 16 * 4
+    for ws, n in ((None, need), (4096, need - 1), (4096 + 128, need)):
+        assert lib.wm_product(C.byref(d), ws, n, None) == -2
+    d = desc(inn=7, ldx=7, ldw=7, rows=40, x_rows=40)                                # odd rows: copies
+    assert lib.wm_product_workspace_size(C.byref(d), 0) >= (40 + 16) * 8 * 2
+    d.dz, d.ld_dz = 4096, 16
+    assert lib.wm_product_workspace_size(C.byref(d), 1) >= (40 + 16) * 8 * 2
+    assert lib.wm_product_backward(C.byref(d), 4096, 7, None, 0, None, None, 0, None) == -2
+    p = C.c_int()
+    assert lib.wm_product_plan(C.byref(d), 3, C.byref(p)) == -2 and lib.wm_product_plan(C.byref(d), 0, None) == -2

@@ -94,6 +94,59 @@ def test_linear_backward(dense, size, dt):
     ref.within(only[2], d64.sum(0), (T + 2) * 2.0 ** -23 * d64.abs().sum(0), "db alone")
 
 
+def mm64(a, b):
+    """(a b, |a| |b|) in 64 bits on the device."""
+    a, b = a.double(), b.double()
+    return torch.mm(a, b).cpu(), torch.mm(a.abs(), b.abs()).cpu()
+
+
+@pytest.mark.parametrize("direction", ["forward", "dx", "dw"])
+def test_every_kernel(dense, direction):
+    """KERNEL_SHAPES, even groups with an empty one, ragged tokens: each kernel, whole and in parts, against 64 bits."""
+    for n, (R, K, N, E) in enumerate(ref.KERNEL_SHAPES[direction]):
+        dt = DT[n % 2]
+        case("every kernel", direction, R, K, N, E, dt)
+        x, w, dz = rnd(80, R, K, dt=dt), rnd(81, E, N, K, dt=dt, scale=0.1), rnd(82, R, N, dt=dt, scale=0.1)
+        cut = [0, *(R * e // E for e in range(1, E)), R]
+        if E > 2:
+            cut[1] = 0                                      # the first expert gets nothing
+        off = torch.tensor(cut, dtype=torch.int32, device="cuda") if E > 1 else None
+        tok = torch.randperm(R, generator=torch.Generator().manual_seed(n)).int().cuda() if E > 1 and n % 3 else None
+        xg = x if tok is None else x[tok.long()]
+        b = rnd(83, E, N, dt=dt)
+        if direction == "forward":
+            y = (dense.linear(x, w[0], bias=b[0]) if E == 1 else
+                 dense.grouped_matmul(x, w, off, token=tok, bias=b, out=torch.zeros(R, N, dtype=dt, device="cuda")))
+            gated = (dense.linear(x, w[0], act="swiglu", out_dtype=F32) if E == 1 else
+                     dense.grouped_matmul(x, w, off, token=tok, act="swiglu", out_dtype=F32)) if N % 2 == 0 else None
+        elif E == 1:
+            dx, dw, db = dense.linear_backward(dz, x, w[0], need_db=direction == "dw", need_dx=direction == "dx",
+                                               need_dw=direction == "dw", dw_dtype=F32 if n % 2 else dt)
+        else:
+            dx, dw, db = dense.grouped_matmul_backward(dz, x, w, off, token=tok, need_db=direction == "dw", need_dx=direction == "dx",
+                                                       need_dw=direction == "dw", dw_dtype=F32 if n % 2 else dt)
+        for e in range(E):
+            r = slice(cut[e], cut[e + 1])
+            rows = r.stop - r.start
+            what = f"{direction} {(R, K, N, E)} group {e}"
+            if direction == "forward" and rows:
+                z, mag = mm64(xg[r], w[e].T)
+                bias = b[e].double().cpu()
+                ref.within(y[r], z + bias, (K + 3) * 2.0 ** -23 * (mag + bias.abs()), what)
+                if gated is not None:
+                    (g, u), (dg, du) = z.chunk(2, 1), ((K + 2) * 2.0 ** -23 * mag).chunk(2, 1)
+                    s = g * torch.sigmoid(g)
+                    ref.within(gated[r], s * u, 1.1 * dg * (u.abs() + du) + s.abs() * du + 2.0 ** -20 * (s * u).abs(), what + " swiglu")
+            elif direction == "dx" and rows:
+                want, mag = mm64(dz[r], w[e])
+                ref.within(dx[r], want, (N + 2) * 2.0 ** -23 * mag, what)
+            elif direction == "dw":
+                want, mag = mm64(dz[r].T.contiguous(), xg[r])
+                ref.within(dw if E == 1 else dw[e], want, (rows + 2) * 2.0 ** -23 * mag, what)
+                d64 = dz[r].double().cpu()
+                ref.within(db if E == 1 else db[e], d64.sum(0), (rows + 2) * 2.0 ** -23 * d64.abs().sum(0), what + " db")
+
+
 def test_linear_extremes(dense):
     """Infinities and NaN stay in their row and column, also next to a ragged end."""
     for T, K, N in ((5, 70, 19), (150, 70, 150)):
@@ -487,3 +540,43 @@ def test_captured_and_replayed(dense):
         torch.cuda.synchronize()
         for i, (a, b) in enumerate(zip(held, want)):
             assert torch.equal(a, b), (n, i)
+
+
+def test_two_streams_at_once(dense):
+    """The same products, in parts and whole, on two streams together: each keeps its own workspace."""
+    cases = [(rnd(90, 1000, 2056), rnd(91, 16, 2056, scale=0.1)), (rnd(92, 40, 71), rnd(93, 57, 71, scale=0.1)),
+             (rnd(94, 600, 1024), rnd(95, 512, 1024, scale=0.1))]
+    want = [(dense.linear(x, w), *dense.linear_backward(rnd(96, x.shape[0], w.shape[0]), x, w, need_db=True)) for x, w in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    dz = [rnd(96, x.shape[0], w.shape[0]) for x, w in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for s, keep in zip(streams, got):
+            for (x, w), g in zip(cases, dz):
+                with torch.cuda.stream(s):
+                    keep.append((dense.linear(x, w), *dense.linear_backward(g, x, w, need_db=True)))
+    torch.cuda.synchronize()
+    for keep in got:
+        for i, r in enumerate(keep):
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i % len(cases)]))
+
+
+def test_parts_and_copies_captured(dense):
+    """A product in parts and one whose operands are copied, under a graph, replayed between eager calls."""
+    x, w, dz = rnd(97, 1000, 2055), rnd(98, 16, 2055, scale=0.1), rnd(99, 1000, 16)
+    step = lambda: (dense.linear(x, w, act="silu"), *dense.linear_backward(dz, x, w, need_db=True, dw_dtype=F32))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for n in range(4):
+        x.copy_(rnd(100 + n, 1000, 2055))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), n
