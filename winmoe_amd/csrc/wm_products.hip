@@ -253,6 +253,30 @@ WM_DEV void store_tile(const ProductArgs& a, int e, int part, int p0, int q0, in
     }
 }
 
+// dW's fragments straight from the registers, 4 outputs per lane and store:
+// fp32 always (64 bytes of a row per store; 2047 x 4096 over 1001 rows 40.2 us
+// through LDS, 35.6 us so), 16 bits where products take longer than the writes
+// (64 experts' 1024 x 2048 over 16384 rows 236 and 226 us, but 512 experts over
+// 5120 rows 1482 and 1558 us).
+template <bool BF, int FP, int FQ>
+WM_DEV void store_direct(const ProductArgs& a, int e, int p0, int q0, int lane, const f32x4 (&acc)[FP][FQ]) {
+    const int pl = p0 + 4 * (lane >> 4);
+#pragma unroll
+    for (int j = 0; j < FQ; j++) {
+        const int q = q0 + 16 * j + (lane & 15);
+        if (q >= a.out) continue;
+        const int64_t at = ((int64_t)e * a.out + q) * a.in + pl;
+#pragma unroll
+        for (int i = 0; i < FP; i++) {
+            if (pl + 16 * i >= a.in) continue;
+            const f32x4 v = acc[i][j];
+            if (a.dw_f32) *(f32x4*)((float*)a.dw + at + 16 * i) = v;
+            else *(uint2*)((uint16_t*)a.dw + at + 16 * i) = (uint2){to16<BF>(v[0]) | (uint32_t)to16<BF>(v[1]) << 16,
+                                                                  to16<BF>(v[2]) | (uint32_t)to16<BF>(v[3]) << 16};
+        }
+    }
+}
+
 // One output of the forward product, from its sums.
 template <bool BF> WM_DEV void store_one(const ProductArgs& a, int e, int q, int p, int outs, float z, float u) {
     const bool gated = a.act == WM_ACT_SWIGLU;
@@ -506,6 +530,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
         w = a.w + (int64_t)e * a.w_stride;
     }
 
+    const int steps = cn - c0;
     if (a.split > 1) {
         const int n = (cn - c0 + BK - 1) / BK, first = c0;
         c0 = first + BK * (int)((int64_t)n * part / a.split);
@@ -548,19 +573,27 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
             qsrc[i] = a.dz + (q0 + ix < qn ? q0 + ix : q0);
         }
     }
-    // DW gathers rows of x: a load of 64 chunks covers 64 / (BP / 8) rows, whose
-    // tokens come through scalar loads (vector loads would wait for the stages
-    // in flight before them)
-    auto token = [&](int c, int i) __attribute__((always_inline)) {
-        constexpr int R = 512 / BP;
-        const int r = c + (64 * wave + i * NT) / (BP / 8);
-        int t = -1;
+    // DW gathers rows of x: a load of 64 chunks covers R rows.  Their tokens come
+    // through scalar loads (vector loads would wait for the stages in flight
+    // before them), one stage ahead (64 experts, 16384 gathered rows: 226 us
+    // without, 186 us with).
+    constexpr int R = 512 / BP;
+    int tok[NP][R] = {};
+    auto tokens = [&](int c) __attribute__((always_inline)) {
+        if (DIR == DW && a.token)
 #pragma unroll
-        for (int k = 0; k < R; k++) {
-            const int v = r + k < cn ? ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)a.token)[r + k] : -1;
-            t = R == 1 || lane / (64 / R) == k ? v : t;
-        }
-        return t;
+            for (int i = 0; i < NP; i++)
+#pragma unroll
+                for (int k = 0; k < R; k++) {
+                    const int r = c + (64 * wave + i * NT) / (BP / 8) + k;
+                    tok[i][k] = r < cn ? ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)a.token)[r] : -1;
+                }
+    };
+    auto token = [&](int i) __attribute__((always_inline)) {
+        int v = 0;
+#pragma unroll
+        for (int k = 0; k < R; k++) v |= tok[i][k] & -(int)(lane / (64 / R) == k);
+        return v;
     };
     auto fill_p = [&](int c, int i, lds8_t* dst) __attribute__((always_inline)) {
         const int at = c + pc[i];
@@ -568,7 +601,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
         if (PC) {
             src = at < plim[i] ? psrc[i] + at : zero_chunk;
         } else if (DIR == DW) {
-            const int t = a.token ? token(c, i) : at;
+            const int t = a.token ? token(i) : at;
             src = at < cn && (uint32_t)t < (uint32_t)a.x_rows ? psrc[i] + (int64_t)t * a.ldx : zero_chunk;
         } else {
             src = at < cn ? psrc[i] + (int64_t)at * a.ldw : zero_chunk;
@@ -690,8 +723,10 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
 #pragma unroll
         for (int i = 0; i < S - 1; i++) {
             if (i && c0 + i * BK >= cn) break;
+            tokens(c0 + i * BK);
             fill(c0 + i * BK, i);
         }
+        tokens(c0 + (S - 1) * BK);
         int b = 0;
         for (int c = c0; c < cn; c += BK) {
             // stages c + BK .. c + (S - 2) BK may still be in flight
@@ -699,6 +734,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
             else WM_WAIT_VMCNT(0);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (c + (S - 1) * BK < cn) fill(c + (S - 1) * BK, b == 0 ? S - 1 : b - 1);
+            tokens(c + S * BK);
             const lds8_t* pt = (const lds8_t*)lds + b * STAGE;
 #pragma unroll
             for (int h = 0; h < BK / 32; h++) {
@@ -711,6 +747,12 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
     }
     if (sums) store_db<FQ>(a, e, part, q0 + wq * (BQ / WQ), lane, sum);
     if (DIR == DW && !a.dw) return;
+    if constexpr (DIR == DW) {
+        if (a.split == 1 && a.in % 4 == 0 && (uintptr_t)a.dw % 16 == 0 && (a.dw_f32 || steps > 2 * BK)) {
+            store_direct<BF, FP, FQ>(a, e, p0 + wp * (BP / WP), q0 + wq * (BQ / WQ), lane, acc);
+            return;
+        }
+    }
     store_tile<BF, DIR, FP, FQ, PH>(a, e, part, p0 + (gated ? wp * (BP / WP / 2) : wp * (BP / WP)), q0 + wq * (BQ / WQ), qn, outs, lane, acc,
                                     (lf32_t*)lds + wave * epilogue_floats<FP, FQ, PH>());
 }
