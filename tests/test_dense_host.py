@@ -158,10 +158,10 @@ def test_workspace_is_asked_for_and_checked(lib):
     assert need >= 2 * 1000 * 16 * 4
     for ws, n in ((None, need), (4096, need - 1), (4096 + 128, need)):
         assert lib.wm_product(C.byref(d), ws, n, None) == -2
-    d = desc(inn=7, ldx=7, ldw=7, rows=40, x_rows=40)                                # odd rows: copies
-    assert lib.wm_product_workspace_size(C.byref(d), 0) >= (40 + 16) * 8 * 2
-    d.dz, d.ld_dz = 4096, 16
-    assert lib.wm_product_workspace_size(C.byref(d), 1) >= (40 + 16) * 8 * 2
-    assert lib.wm_product_backward(C.byref(d), 4096, 7, None, 0, None, None, 0, None) == -2
+    d = desc(inn=1031, ldx=1031, ldw=1031, out=512, ldy=512, rows=4000, x_rows=4000)  # odd rows: copies
+    assert lib.wm_product_workspace_size(C.byref(d), 0) >= (4000 + 512) * 1032 * 2
+    d.dz, d.ld_dz = 4096, 512
+    assert lib.wm_product_workspace_size(C.byref(d), 1) >= (4000 + 512) * 1032 * 2
+    assert lib.wm_product_backward(C.byref(d), 4096, 1031, None, 0, None, None, 0, None) == -2
     p = C.c_int()
     assert lib.wm_product_plan(C.byref(d), 3, C.byref(p)) == -2 and lib.wm_product_plan(C.byref(d), 0, None) == -2

@@ -235,12 +235,16 @@ WM_DEV void store_tile(const ProductArgs& a, int e, int part, int p0, int q0, in
             if (q >= qn || n <= 0) continue;
             // SwiGLU: 16 gate values, then the up values of the same outputs
             const lf32_t* src = lds + r * ROW + (gated ? 32 * (u >> 1) + 8 * (u & 1) : 8 * u);
-            float z[8];
+            const f32x4 lo = *(const lf32x4*)src, hi = *(const lf32x4*)(src + 4);
+            float z[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, up[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (gated) {
+                const f32x4 l = *(const lf32x4*)(src + 16), h = *(const lf32x4*)(src + 20);
 #pragma unroll
-            for (int i = 0; i < 8; i++) z[i] = src[i];
-            float up[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) up[i] = gated ? src[16 + i] : 0.0f;
+                for (int i = 0; i < 4; i++) {
+                    up[i] = l[i];
+                    up[4 + i] = h[i];
+                }
+            }
             if (a.split > 1) {
                 const int64_t at = DIR == DW ? (int64_t)(part * a.E + e) * a.out + q : (int64_t)part * a.rows + q;
                 float* d = a.part + at * (DIR == FWD ? a.out : a.in) + p;
@@ -886,27 +890,28 @@ __global__ __launch_bounds__(256) void k_repack(const uint16_t* __restrict__ src
 
 // ------------------------------------------------------------------ launch
 
-// How a product is run.  The tile kernels' times are estimated from their own
-// measurements (bf16, in 64 stages): `alone` is what a stage of 64 steps takes
-// with one workgroup on a CU, `share` what it adds to a CU that is full, both
-// in us.
+// How a product is run.  The kernels' times are estimated from their own
+// measurements (bf16): `alone` is what a stage of 64 steps takes with one
+// workgroup on a CU, `share` what it adds to a CU that is full, `ends` a tile's
+// first loads and its stores, all in us.
 enum Kernel : int { ANY128, ANY32, FEW, T256, T128, T128x64, T128x32, T64, T64x32, T64x16 };
 struct TileCost {
     Kernel k;
     int bp, bq, resident;
-    float alone, share;
+    float alone, share, ends;
 };
 static constexpr TileCost kTiles[] = {
-    {T256, 256, 256, 1, 1.40f, 1.65f}, {T128, 128, 128, 2, 0.82f, 0.54f},  {T128x64, 128, 64, 2, 0.58f, 0.36f},
-    {T128x32, 128, 32, 2, 0.46f, 0.33f}, {T64, 64, 64, 2, 0.40f, 0.27f},   {T64x32, 64, 32, 3, 0.34f, 0.20f},
-    {T64x16, 64, 16, 4, 0.34f, 0.15f},
+    {T256, 256, 256, 1, 1.40f, 1.65f, 6.0f},  {T128, 128, 128, 2, 0.82f, 0.54f, 3.0f}, {T128x64, 128, 64, 2, 0.58f, 0.36f, 2.5f},
+    {T128x32, 128, 32, 2, 0.40f, 0.33f, 2.0f}, {T64, 64, 64, 2, 0.40f, 0.27f, 2.0f},    {T64x32, 64, 32, 3, 0.34f, 0.20f, 2.0f},
+    {T64x16, 64, 16, 4, 0.34f, 0.15f, 2.0f},   {ANY128, 128, 128, 2, 1.00f, 0.69f, 3.0f}, {ANY32, 128, 32, 4, 0.70f, 0.45f, 2.0f},
 };
 struct Plan {
     Kernel k;
     int split;
 };
+static bool tiled(const Plan& p) { return p.k >= T256; }
 
-static int columns(const ProductArgs& a, int dir) {      // of the result, and of an output tile for SwiGLU
+static int columns(const ProductArgs& a, int dir) {      // of the result
     return dir == FWD ? (a.act == WM_ACT_SWIGLU ? a.out / 2 : a.out) : a.in;
 }
 
@@ -916,68 +921,78 @@ static int64_t row_tiles(const ProductArgs& a, int bq) {
     return std::min((int64_t)a.rows, (int64_t)a.rows / bq + a.E);
 }
 
-// The tile and the number of parts with the least estimated time.  The chip is
-// taken as 256 CUs; the rows of a group are taken as even, as the host does not
-// know them.  Reading the weights (writing, for dW) overlaps the products, but
-// not fully; tiles 64 wide read them in shorter rows.  A split pays a second
-// kernel (which has to look groups up) and the parts' way to memory and back:
-// 4 or 7 us and 2.5 TB/s.
-static Plan plan_tiles(const ProductArgs& a, int dir) {
-    const double groups = a.offsets ? std::max(1.0, std::min((double)a.E, (double)a.rows)) : 1.0, per = a.rows / groups;
-    const int outs = columns(a, dir);
-    const bool gated = dir == FWD && a.act == WM_ACT_SWIGLU;
-    const double steps = dir == FWD ? a.in : dir == DX ? a.out : per;
-    const double stages = std::max(1.0, std::ceil(steps / BK));
-    const double memory = (dir == DW ? a.E * (1.0 + a.dw_f32) : groups) * a.in * a.out * 2.0 / 5.6e6;       // us
-    const double sums = (dir == DW ? (double)a.E * a.out * a.in : (double)a.rows * (dir == FWD ? a.out : a.in)) * 8.0;
-    Plan best{T128, 1};
-    double least = 1e30;
-    for (const TileCost& t : kTiles) {
-        if (dir == DW && t.bp != t.bq) continue;
-        const double p = std::ceil(outs / (double)(gated ? t.bp / 2 : t.bp));
-        const double q = dir == DW ? a.E * std::ceil(a.out / (double)t.bq) : groups > 1 ? groups * (0.5 + std::max(0.5, per / t.bq)) : std::ceil(per / t.bq);
-        for (int s = 1; s <= 16 && s * 2 <= stages + 1; s *= 2) {
-            if (s > 1 && s * sums > 512e6) break;
-            const double n = std::max(1.0, p * q * s / 256), turns = std::max(1.0, n / t.resident);
-            const double work = std::ceil(stages / s) * std::max(t.alone * turns, t.share * n) + 2.0 * turns;
-            const double stream = t.bp < 128 ? 1.15 * memory : memory;
-            const double us = std::max(work, stream) + 0.3 * std::min(work, stream) + (s > 1 ? (a.offsets ? 7.0 : 4.0) + s * sums / 2.5e6 : 0.0);
-            if (us < least) {
-                least = us;
-                best = {t.k, s};
-            }
-        }
-    }
-    return best;
-}
-
 // Whether every 16-byte chunk of an operand is aligned and whole.
 static bool chunks16(const void* p, int64_t ld, int cols) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && cols % 8 == 0; }
 
-// What is copied before the tile kernels: operands of odd or unaligned rows.
+// What the LDS-DMA tiles need copied first: operands of odd or unaligned rows.
 struct Copies {
     bool x, w, dz;
+    bool any() const { return x || w || dz; }
 };
 static Copies copies(const ProductArgs& a, bool fwd, bool dx, bool dw) {
     return {(fwd || dw) && !chunks16(a.x, a.ldx, a.in), (fwd || dx) && !(chunks16(a.w, a.ldw, a.in) && a.w_stride % 8 == 0),
             (dx || dw) && !chunks16(a.dz, a.lddz, a.out)};
 }
 
-// Which kernel takes a forward product (or dx) whose operands need copies, or
-// of few rows.
-//   FEW (forward, up to 16 rows in all, or in a group where copies would be
-//   needed): one launch, 4096 x 4096 weights and one row 9.5 us against 12.4 us
-//   of split tiles; 16 rows and 65536 outputs 128 us against 101 us, so with
-//   many rows only where W is small.
-//   ANY32 (any alignment): groups of under 64 rows whose weights would have to
-//   be copied; they are bound by reading the weights, a copy would read and
-//   write them once more.
-static Plan plan_rows(const ProductArgs& a, int dir) {
-    const int64_t per = a.rows / a.E;
-    const bool odd = dir == FWD ? copies(a, true, false, false).w : copies(a, false, true, false).w;
-    if (dir == FWD && !a.offsets && a.rows <= 16 && (odd || a.rows <= 4 || (int64_t)a.in * a.out <= 1 << 25)) return {FEW, 1};
-    if (odd && a.offsets && per < 64) return {dir == FWD && per <= 2 ? FEW : ANY32, 1};
-    return plan_tiles(a, dir);
+// The kernel and the number of parts with the least estimated time.  The chip
+// is taken as 256 CUs.  The host does not know the groups: rows are taken as
+// spread evenly at random over the experts, with some more tiles than that
+// makes, as groups are skewed.
+//
+// Tiles: reading the weights (writing, for dW) overlaps the products, the worse
+// the closer the two are; tiles 64 wide read them in shorter rows.  A split pays a second kernel
+// (which has to look groups up) and the parts' way to memory and back: 4 or 7 us
+// and 2.5 TB/s.  Copies pay 3 us and 4 TB/s, which the kernels for any alignment
+// do not need.
+// Few rows (k_product_few, forward): W once per 16 rows, 5.2 TB/s (grouped 4.6,
+// and up to 1024 columns 3.9, where workgroups are short), x from the caches at
+// 15 TB/s, or the time of its waves' batches one after another.  In a graph, us: 1 row,
+// 4096 x 4096 9.0 (split tiles 12.4); 48 rows 25 (tiles 14.5); 4 of 64 experts'
+// 1024 x 2048 7.3 (tiles 18.3); 16 rows, 65536 x 4096 122 (tiles 110).
+static Plan plan(const ProductArgs& a, int dir) {
+    const double E = a.E, rows = a.rows, groups = a.offsets && E > 1 ? std::max(1.0, E * (1.0 - std::exp(-rows / E))) : 1.0, per = rows / groups;
+    const int outs = columns(a, dir);
+    const bool gated = dir == FWD && a.act == WM_ACT_SWIGLU;
+    const double stages = std::max(1.0, std::ceil((dir == FWD ? a.in : dir == DX ? a.out : per) / BK));
+    const double weights = 2.0 * groups * a.in * a.out;
+    const double memory = (dir == DW ? 2.0 * E * a.in * a.out * (1.0 + a.dw_f32) : weights) / 5.6e6;        // us
+    const double sums = (dir == DW ? E * a.out * a.in : rows * (dir == FWD ? a.out : a.in)) * 8.0;
+    const Copies c = copies(a, dir == FWD, dir == DX, dir == DW);
+    double copy = 0.0;
+    if (c.w) copy += 3.0 + 4.0 * E * a.in * a.out / 4e6;
+    if (c.x) copy += 3.0 + 4.0 * a.x_rows * a.in / 4e6;
+    if (c.dz) copy += 3.0 + 4.0 * rows * a.out / 4e6;
+    auto row_parts = [&](int bq) { return groups > 1 ? groups * (0.75 + std::max(0.25, per / bq)) : std::ceil(rows / bq); };
+
+    Plan best{T128, 1};
+    double least = 1e30;
+    for (const TileCost& t : kTiles) {
+        const bool any = t.k == ANY128 || t.k == ANY32;
+        if ((dir == DW && (any || t.bp != t.bq)) || (any && !c.any())) continue;
+        const double p = std::ceil(outs / (double)(gated ? t.bp / 2 : t.bp));
+        const double q = dir == DW ? E * std::ceil(a.out / (double)t.bq) : row_parts(t.bq);
+        for (int s = 1; s <= (any ? 1 : 16) && s * 2 <= stages + 1; s *= 2) {
+            if (s > 1 && s * sums > 512e6) break;
+            const double n = std::ceil(p * q * s / 256), turns = std::max(1.0, n / t.resident);
+            const double work = std::ceil(stages / s) * std::max(t.alone * turns, t.share * n) + t.ends * turns;
+            const double stream = t.bp < 128 ? 1.15 * memory : memory;
+            const double more = std::max(work, stream), less = std::min(work, stream);
+            const double us = 3.0 + more + 0.35 * less * (less / more) * (less / more) + (any ? 0.0 : copy) +
+                              (s > 1 ? (a.offsets ? 7.0 : 4.0) + s * sums / 2.5e6 : 0.0);
+            if (us < least) {
+                least = us;
+                best = {t.k, s};
+            }
+        }
+    }
+    if (dir == FWD) {
+        const double passes = row_parts(16) / groups, x = row_parts(16) * std::min(per, 16.0) * a.in * 2.0 * std::ceil(outs / (gated ? 8.0 : 16.0));
+        const double batches = std::ceil(a.in / (a.in <= 2048 ? 4.0 : 8.0) / 64) / 4;           // of 8 loads, per wave
+        const double rate = a.in <= 1024 ? 3.9e6 : a.offsets ? 4.6e6 : 5.2e6;
+        const double us = (a.offsets ? 5.5 : 3.0) + std::max(passes * weights / rate + x / 15e6, batches * (1.6 + 0.085 * std::min(per, 16.0)));
+        if (us < least) best = {FEW, 1};
+    }
+    return best;
 }
 
 struct Layout {
@@ -999,8 +1014,6 @@ static int64_t part_bytes(const ProductArgs& a, int dir, int split) {
     const int64_t n = dir == DW ? (int64_t)a.E * a.out * (a.in + 1) : (int64_t)a.rows * (dir == FWD ? a.out : a.in);
     return 4 * n * split;
 }
-static bool tiled(const Plan& p) { return p.k >= T256; }
-
 // db without dw takes one column of x.
 static ProductArgs without_dx(const ProductArgs& a) {
     ProductArgs b = a;
@@ -1009,7 +1022,7 @@ static ProductArgs without_dx(const ProductArgs& a) {
 }
 
 int product_plan(const ProductArgs& a, int dir, int* parts) {
-    const Plan p = dir == DW ? plan_tiles(a, DW) : plan_rows(a, dir);
+    const Plan p = plan(a, dir);
     *parts = p.split;
     return p.k;
 }
@@ -1017,20 +1030,20 @@ int product_plan(const ProductArgs& a, int dir, int* parts) {
 int64_t product_workspace(const ProductArgs& a, bool backward) {
     if (a.rows == 0) return 0;
     if (!backward) {
-        const Plan p = plan_rows(a, FWD);
+        const Plan p = plan(a, FWD);
         return layout(a, tiled(p) ? copies(a, true, false, false) : Copies{}, part_bytes(a, FWD, p.split)).total;
     }
     // whichever of dx, dw and db the call asks for
     ProductArgs b = a;
     int64_t part = 0;
-    const Plan px = plan_rows(a, DX);
+    const Plan px = plan(a, DX);
     part = part_bytes(a, DX, px.split);
     for (int f32 = 0; f32 < 2; f32++) {
         b.dw_f32 = f32;
-        part = std::max(part, part_bytes(b, DW, plan_tiles(b, DW).split));
+        part = std::max(part, part_bytes(b, DW, plan(b, DW).split));
     }
     b.in = 1;
-    part = std::max(part, part_bytes(b, DW, plan_tiles(b, DW).split));
+    part = std::max(part, part_bytes(b, DW, plan(b, DW).split));
     return layout(a, copies(a, false, tiled(px), true), part).total;
 }
 
@@ -1066,6 +1079,7 @@ template <int DIR> static int run_tiles(const ProductArgs& a, Kernel k, hipStrea
         case T128x32: return run<DIR, 128, 32, 4, 1, 4>(a, s);
         case T64x32: return run<DIR, 64, 32, 2, 2, 4>(a, s);
         case T64x16: return run<DIR, 64, 16, 2, 1, 4>(a, s);
+        case ANY128: return run<DIR, 128, 128, 2, 2, 0>(a, s);
         case ANY32: return run<DIR, 128, 32, 4, 1, 0>(a, s);
         default: break;
         }
@@ -1117,7 +1131,7 @@ static int copy_operands(ProductArgs& a, const Copies& c, const Layout& l, uint8
 
 int launch_product(const ProductArgs& args, uint8_t* ws, hipStream_t s) {
     ProductArgs a = args;
-    const Plan p = plan_rows(a, FWD);
+    const Plan p = plan(a, FWD);
     a.split = p.split;
     if (p.k == FEW) return a.in <= 2048 ? run_few<4>(a, s) : run_few<8>(a, s);
     const Copies c = tiled(p) ? copies(a, true, false, false) : Copies{};
@@ -1130,7 +1144,7 @@ int launch_product(const ProductArgs& args, uint8_t* ws, hipStream_t s) {
 int launch_product_backward(const ProductArgs& args, uint8_t* ws, hipStream_t s) {
     ProductArgs a = args;
     const bool dx = a.dx && a.rows, dw = a.dw || a.db;
-    const Plan px = dx ? plan_rows(a, DX) : Plan{ANY32, 1};
+    const Plan px = dx ? plan(a, DX) : Plan{ANY32, 1};
     const Copies c = copies(a, false, tiled(px), dw && a.rows);
     const Layout l = layout(a, c, 0);
     ProductArgs b = a;
@@ -1143,7 +1157,7 @@ int launch_product_backward(const ProductArgs& args, uint8_t* ws, hipStream_t s)
     }
     if (dw) {
         ProductArgs t = without_dx(b);
-        const Plan p = a.rows ? plan_tiles(t, DW) : Plan{T128, 1};
+        const Plan p = a.rows ? plan(t, DW) : Plan{T128, 1};
         t.split = p.split;
         t.part_db = t.part + (int64_t)p.split * t.E * t.out * t.in;
         return run_tiles<DW>(t, p.k, s);
