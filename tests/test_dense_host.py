@@ -153,9 +153,11 @@ def test_kernel_shapes_run_every_kernel(lib):
 
 def test_workspace_is_asked_for_and_checked(lib):
     """A call whose size query is not 0 refuses a missing, short or unaligned workspace."""
-    d = desc(rows=1000, x_rows=1000, inn=2056, out=16, ldx=2056, ldw=2056)          # in parts
+    parts = []
+    plan(lib, 3000, 4104, 136, 1, 0, parts)
+    d = desc(rows=3000, x_rows=3000, inn=4104, out=136, ldx=4104, ldw=4104, ldy=136)
     need = lib.wm_product_workspace_size(C.byref(d), 0)
-    assert need >= 2 * 1000 * 16 * 4
+    assert parts[0] > 1 and need >= parts[0] * 3000 * 136 * 4
     for ws, n in ((None, need), (4096, need - 1), (4096 + 128, need)):
         assert lib.wm_product(C.byref(d), ws, n, None) == -2
     d = desc(inn=1031, ldx=1031, ldw=1031, out=512, ldy=512, rows=4000, x_rows=4000)  # odd rows: copies
