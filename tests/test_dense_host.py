@@ -160,10 +160,10 @@ def test_workspace_is_asked_for_and_checked(lib):
     assert parts[0] > 1 and need >= parts[0] * 3000 * 136 * 4
     for ws, n in ((None, need), (4096, need - 1), (4096 + 128, need)):
         assert lib.wm_product(C.byref(d), ws, n, None) == -2
-    d = desc(inn=4095, ldx=4095, ldw=4095, out=2048, ldy=2048, rows=4000, x_rows=4000)  # odd rows: copies
-    assert lib.wm_product_workspace_size(C.byref(d), 0) >= (4000 + 2048) * 4096 * 2
-    d.dz, d.ld_dz = 4096, 2048
-    assert lib.wm_product_workspace_size(C.byref(d), 1) >= (4000 + 2048) * 4096 * 2
+    d = desc(inn=4095, ldx=4095, ldw=4095, out=8192, ldy=8192, rows=4000, x_rows=4000)  # odd rows: copies
+    assert lib.wm_product_workspace_size(C.byref(d), 0) >= (4000 + 8192) * 4096 * 2
+    d.dz, d.ld_dz = 4096, 8192
+    assert lib.wm_product_workspace_size(C.byref(d), 1) >= (4000 + 8192) * 4096 * 2
     assert lib.wm_product_backward(C.byref(d), 4096, 4095, None, 0, None, None, 0, None) == -2
     p = C.c_int()
     assert lib.wm_product_plan(C.byref(d), 3, C.byref(p)) == -2 and lib.wm_product_plan(C.byref(d), 0, None) == -2
