@@ -280,7 +280,8 @@ int64_t wm_expert_workspace_size(int H, int I);
  * inputs, except that residual may be y itself (same ld and type).
  *
  * Groups: rows offsets[e] <= r < offsets[e + 1] belong to expert e (device
- * int32 [n_groups + 1], not decreasing; wm_group_by_expert makes them).  Groups
+ * int32 [n_groups + 1], not decreasing, up to 65535 groups; wm_group_by_expert
+ * makes them).  Groups
  * may be empty.  Rows before the first and behind the last group are neither
  * read nor written.  Offsets outside [0, rows] are taken as the nearer bound,
  * so no memory outside the rows is touched whatever they hold. */
@@ -357,14 +358,14 @@ int wm_act_backward(int dtype, int act, int64_t rows, int cols, const void* dy, 
 /* Sorts T * K picks by expert, stably: ids int32 [T][K] (device).  offsets
  * [E + 1]; token [T * K]: the token of each sorted row; row [T][K]: the sorted
  * row of each pick.  A pick outside [0, E) belongs to no expert: its row is -1,
- * and token is -1 from offsets[E] on.  T * K < 2^31 - 2^16. */
+ * and token is -1 from offsets[E] on.  T * K < 2^31 - 2^16, E < 2^16. */
 int wm_group_by_expert(const int32_t* ids, int T, int K, int E, int32_t* offsets, int32_t* token, int32_t* row,
                        void* stream);
 
 /* out[t] = sum_k w[t][k] * y[row[t][k]] + residual[t], k in order: y [rows][H]
  * (dtype), row int32 [T][K], w fp32 [T][K] or NULL (ones), residual and out
  * [T][H] of out_type (dtype or WM_F32), residual NULL or out itself.  A row
- * outside [0, rows) adds nothing, whatever its weight. */
+ * outside [0, rows) adds nothing, whatever its weight.  T < 2^24. */
 int wm_combine_rows(int dtype, const void* y, int64_t ld_y, int rows, const int32_t* row, const float* w, int T, int K,
                     int H, const void* residual, int64_t ld_residual, void* out, int64_t ld_out, int out_type,
                     void* stream);
@@ -372,7 +373,8 @@ int wm_combine_rows(int dtype, const void* y, int64_t ld_y, int rows, const int3
 /* Its gradients, given dout [T][H] (dout_type: dtype or WM_F32): dy[row[t][k]]
  * = w[t][k] * dout[t] (dtype; rows that no pick names are left as they are)
  * and dw[t][k] = <dout[t], y[row[t][k]]> (fp32; 0 where the row is outside
- * [0, rows)).  dy or dw may be NULL; a row may be named by one pick only. */
+ * [0, rows)).  dy or dw may be NULL; a row may be named by one pick only.
+ * T * ceil(K / 5) < 2^23. */
 int wm_combine_rows_backward(int dtype, const void* dout, int64_t ld_dout, int dout_type, const void* y, int64_t ld_y,
                              int rows, const int32_t* row, const float* w, int T, int K, int H, void* dy,
                              int64_t ld_dy, float* dw, void* stream);

@@ -167,3 +167,36 @@ def test_workspace_is_asked_for_and_checked(lib):
     assert lib.wm_product_backward(C.byref(d), 4096, 4095, None, 0, None, None, 0, None) == -2
     p = C.c_int()
     assert lib.wm_product_plan(C.byref(d), 3, C.byref(p)) == -2 and lib.wm_product_plan(C.byref(d), 0, None) == -2
+
+
+@pytest.mark.parametrize("kw", [dict(n_groups=1 << 16, offsets=64, w_stride=1 << 20), dict(ldw=(1 << 40) + 1),
+                                dict(ldx=(1 << 40) + 1), dict(inn=1 << 26, out=1 << 26, ldx=1 << 26, ldw=1 << 26, ldy=1 << 26)],
+                         ids=str)
+def test_sizes_beyond_any_memory_are_refused(lib, kw):
+    d = desc(**kw)
+    assert lib.wm_product(C.byref(d), None, 0, None) == -2
+    assert lib.wm_product_workspace_size(C.byref(d), 0) < 0
+
+
+def test_combine_refuses_more_tokens_than_a_launch_holds(lib):
+    T = 1 << 24
+    assert lib.wm_combine_rows(30, 4096, 8, 4, 64, None, T, 1, 8, None, 0, 8192, 8, 30, None) == -2
+    for t, k in ((T // 2, 5), (T // 4, 6)):
+        assert lib.wm_combine_rows_backward(30, 4096, 8, 30, 8192, 8, 4, 64, None, t, k, 8, 16384, 8, 64, None) == -2
+
+
+@pytest.mark.parametrize("E, rows, out, inn", [(1, 65536, 64, 8), (3, 10000, 100, 64), (1, 4096, 262144, 8), (64, 2000, 16, 256)])
+def test_workspace_covers_a_bias_gradient_alone(lib, E, rows, out, inn):
+    """db without dw is a product with one column of x, in parts of its own."""
+    d = desc(n_groups=E, offsets=64 if E > 1 else None, rows=rows, x_rows=rows, inn=inn, out=out, ldx=inn, ldw=inn, ldy=out,
+             w_stride=out * inn)
+    d.dz, d.ld_dz = 1 << 20, out
+    one = _copy(d)
+    one.inn = 1
+    parts = C.c_int()
+    assert lib.wm_product_plan(C.byref(one), 2, C.byref(parts)) >= 0
+    assert parts.value == 1 or lib.wm_product_workspace_size(C.byref(d), 1) >= 4 * E * out * 2 * parts.value
+
+
+def _copy(d):
+    return type(d).from_buffer_copy(d)

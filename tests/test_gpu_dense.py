@@ -509,6 +509,20 @@ def test_on_another_stream(dense):
     assert torch.equal(got, want) and torch.equal(also, want)
 
 
+def test_memory_of_the_current_stream_is_not_written_on_another(dense):
+    """What a call on another stream writes does not lie where the current stream may still be reading."""
+    x, w = rnd(62, 300, 512), rnd(63, 384, 512, scale=0.1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    held = torch.empty(300, 384, dtype=x.dtype, device="cuda")
+    at = held.data_ptr()
+    del held                                                # its last use may still be queued
+    got = dense.linear(x, w, stream=s)
+    assert got.data_ptr() != at
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, dense.linear(x, w))
+
+
 def test_captured_and_replayed(dense):
     """The block and its gradients under a graph: every replay, with eager work between, gives the eager bits."""
     T, K, E, H, I = 37, 3, 6, 128, 64

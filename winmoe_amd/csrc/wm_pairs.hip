@@ -23,9 +23,10 @@ namespace wm {
 // the places of its experts' ids in order.  The experts are 0 .. E, the last
 // one standing for the ids outside [0, E): their rows follow the last group.
 //
-// 512 experts: 10 ids 4.5 us, 5120 ids 7 us, 40960 ids 14 us in a graph, of
-// which about 2.4 us is the launch; one expert per workgroup took 4.7, 7.6
-// and 29.6 us.
+// Bound by latency: two rounds of loads, one exchange.  512 experts: 10 ids
+// 3.9 us, 5120 ids 5.9 us, 40960 ids 12.9 us in a graph, of which about 2.4 us
+// is the launch; one id per lane and load and one expert per workgroup took
+// 4.7, 7.6 and 29.6 us.
 constexpr int GRP_WAVES = 16;
 template <int EP> __global__ __launch_bounds__(64 * GRP_WAVES) void k_group(const int32_t* __restrict__ ids, int n, int K, int E,
                                                                             int32_t* __restrict__ offsets, int32_t* __restrict__ token,
@@ -163,7 +164,7 @@ template <bool BF> __global__ __launch_bounds__(256) void k_act_backward(const A
 int launch_act_backward(const ActArgs& a, hipStream_t s) {
     const int64_t blocks = (a.rows * ((a.out + 7) / 8) + 255) / 256;
     if (blocks == 0) return 0;
-    if (blocks > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
+    if (blocks > 0xFFFFFFFFll / 256) return (int)hipErrorInvalidConfiguration;       // a launch holds fewer than 2^32 threads
     if (a.bf16) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_act_backward<true>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_act_backward<false>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
     return (int)hipGetLastError();
@@ -212,6 +213,7 @@ template <bool BF> __global__ __launch_bounds__(256) void k_combine_rows(const C
 
 int launch_combine_rows(const CombineRowsArgs& a, hipStream_t s) {
     if (a.T == 0 || a.H == 0) return 0;
+    if (a.T > 0xFFFFFFFFll / 256) return (int)hipErrorInvalidConfiguration;
     const dim3 grid(a.T, (a.H + 2047) / 2048);
     if (a.bf16) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_combine_rows<true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_combine_rows<false>), grid, dim3(256), 0, s, a);
@@ -291,6 +293,7 @@ int launch_combine_rows_backward(const CombineRowsArgs& a, hipStream_t s) {
     const int per = (a.K + CB - 1) / CB;
     const int64_t blocks = (int64_t)a.T * per;
     if (blocks == 0) return 0;
+    if (blocks > 0xFFFFFFFFll / 512) return (int)hipErrorInvalidConfiguration;
     const auto k = a.bf16 ? k_combine_rows_backward<true> : k_combine_rows_backward<false>;
     // 8 columns per thread: a row of up to 4096 in one go
     hipLaunchKernelGGL(k, dim3((uint32_t)blocks), dim3(a.H > 2048 ? 512 : 256), 0, s, a, per);

@@ -123,11 +123,11 @@ WM_DEV TileId tile_id(int block, int blocks, int nP) {
 
 // ------------------------------------------------------------------ LDS tiles
 
-// [TILE][KB], memory rows along the contraction.  A row's 16-byte chunks are
+// [TILE][BK], memory rows along the contraction.  A row's 16-byte chunks are
 // permuted by its index, so that the 16 rows of a read fall on all banks.
-template <int TILE, int KB> struct AlongC {
-    static constexpr int CH = KB / 8;
-    WM_DEV static int perm(int index) { return KB == 64 ? index & 7 : (index >> 1) & 3; }
+template <int TILE> struct AlongC {
+    static constexpr int CH = BK / 8;
+    WM_DEV static int perm(int index) { return index & 7; }
     // what slot s (16 bytes) holds
     WM_DEV static void slot(int s, int& index, int& c) {
         index = s / CH;
@@ -136,14 +136,14 @@ template <int TILE, int KB> struct AlongC {
     // operand of 16 indices from `base` on, 32 contraction steps from 32 * ks on
     WM_DEV static s16x8 frag(const lds8_t* t, int base, int ks, int lane) {
         const int i = base + (lane & 15), ch = (4 * ks + (lane >> 4)) ^ perm(lane & 15);
-        return *(const __attribute__((address_space(3))) s16x8*)(t + 2 * KB * i + 16 * ch);
+        return *(const __attribute__((address_space(3))) s16x8*)(t + 2 * BK * i + 16 * ch);
     }
 };
 
-// [KB][TILE], memory rows are contraction steps.  Units of 16 values are
+// [BK][TILE], memory rows are contraction steps.  Units of 16 values are
 // permuted within a row by the row's bits 0, 1 and 3, which the 16 rows of a
 // transposing read run through.
-template <int TILE, int KB> struct AcrossC {
+template <int TILE> struct AcrossC {
     static constexpr int CH = TILE / 8, U = TILE / 16;
     WM_DEV static int perm(int c) { return ((c & 3) | ((c >> 1) & 4)) & (U - 1); }
     WM_DEV static void slot(int s, int& index, int& c) {
@@ -328,9 +328,10 @@ template <bool BF, int DIR, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     constexpr int NT = 64 * WP * WQ, FP = BP / WP / 16, FQ = BQ / WQ / 16;
     static_assert(DIR != FWD || FP % 2 == 0, "SwiGLU's gate and up meet in a wave");
-    constexpr bool PC = DIR == FWD, QC = DIR != DW;         // operand's rows run along the contraction
-    using PT = typename std::conditional<PC, AlongC<BP, BK>, AcrossC<BP, BK>>::type;
-    using QT = typename std::conditional<QC, AlongC<BQ, BK>, AcrossC<BQ, BK>>::type;
+    static_assert(DIR != DW, "dW runs on copies");
+    constexpr bool PC = DIR == FWD;         // W's rows run along the contraction; x's and dz's do
+    using PT = typename std::conditional<PC, AlongC<BP>, AcrossC<BP>>::type;
+    using QT = AlongC<BQ>;
     constexpr int PS = BP * 8, QS = BQ * 8, NP = (PS + NT - 1) / NT, NQ = (QS + NT - 1) / NT;
     constexpr int STAGE = (BP + BQ) * 2 * BK, PH = 1, EPI = WP * WQ * 4 * epilogue_floats<FP, FQ, PH>();
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE > EPI ? 2 * STAGE : EPI];
@@ -342,25 +343,10 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     const int cols = gated ? BP / 2 : BP;
     const int nP = (outs + cols - 1) / cols;
     const int p0 = (int)(blockIdx.x % nP) * cols;
-    int e, q0, qn, c0 = 0, cn;
-    const uint16_t* w;
-    if (DIR == DW) {
-        const int nQ = (a.out + BQ - 1) / BQ, t = blockIdx.x / nP;
-        e = t / nQ;
-        q0 = (t % nQ) * BQ;
-        qn = a.out;
-        c0 = a.offsets ? min(max(a.offsets[e], 0), a.rows) : 0;
-        cn = a.offsets ? min(max(a.offsets[e + 1], c0), a.rows) : a.rows;       // contraction [c0, cn)
-        w = nullptr;
-    } else {
-        const GroupTile g = find_tile(a.offsets, a.E, a.rows, BQ, blockIdx.x / nP);
-        if (g.e < 0) return;
-        e = g.e;
-        q0 = g.start + g.tile * BQ;
-        qn = g.start + g.n;
-        cn = DIR == FWD ? a.in : a.out;
-        w = a.w + (int64_t)e * a.w_stride;
-    }
+    const GroupTile g = find_tile(a.offsets, a.E, a.rows, BQ, blockIdx.x / nP);
+    if (g.e < 0) return;
+    const int e = g.e, q0 = g.start + g.tile * BQ, qn = g.start + g.n, cn = DIR == FWD ? a.in : a.out;
+    const uint16_t* w = a.w + (int64_t)e * a.w_stride;
     // row of x of grouped row r, or none
     auto xrow = [&](int r) __attribute__((always_inline)) -> const uint16_t* {
         const int t = a.token ? a.token[r] : r;
@@ -384,7 +370,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     for (int i = 0; i < NQ; i++) {
         QT::slot(tid + i * NT, qi[i], qc[i]);
         qrow[i] = nullptr;
-        if (QC && tid + i * NT < QS && q0 + qi[i] < qn) {
+        if (tid + i * NT < QS && q0 + qi[i] < qn) {
             const int r = q0 + qi[i];
             qrow[i] = DIR == FWD ? xrow(r) : a.dz + (int64_t)r * a.lddz;
         }
@@ -398,20 +384,11 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
             } else {
                 const int r = c + pc[i];
                 const bool live = r < cn && tid + i * NT < PS;
-                const uint16_t* row = !live ? nullptr : DIR == DW ? xrow(r) : w + (int64_t)r * a.ldw;
-                pv[i] = load8(row + p0 + pi[i], row ? outs - p0 - pi[i] : 0);
+                pv[i] = load8(w + (int64_t)r * a.ldw + p0 + pi[i], live ? outs - p0 - pi[i] : 0);
             }
         }
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            if (QC) {
-                qv[i] = load8(qrow[i] + c + qc[i], qrow[i] ? cn - c - qc[i] : 0);
-            } else {
-                const int r = c + qc[i];
-                const bool live = r < cn && tid + i * NT < QS;
-                qv[i] = load8(a.dz + (int64_t)r * a.lddz + q0 + qi[i], live ? a.out - q0 - qi[i] : 0);
-            }
-        }
+        for (int i = 0; i < NQ; i++) qv[i] = load8(qrow[i] + c + qc[i], qrow[i] ? cn - c - qc[i] : 0);
     };
     auto stage = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
@@ -423,23 +400,16 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
     };
 
     f32x4 acc[FP][FQ];
-    float sum[FQ];
 #pragma unroll
     for (int i = 0; i < FP; i++)
 #pragma unroll
         for (int j = 0; j < FQ; j++) acc[i][j] = (f32x4)0.0f;
-#pragma unroll
-    for (int j = 0; j < FQ; j++) sum[j] = 0.0f;
-    // db: the first tile of p sums the operand that it reads anyway
-    const bool sums = DIR == DW && a.db && p0 == 0 && wp == 0;
 
-    if (c0 < cn) {
-        load(c0);
-        stage(0);
-        __syncthreads();
-    }
+    load(0);
+    stage(0);
+    __syncthreads();
     int b = 0;
-    for (int c = c0; c < cn; c += BK, b ^= 1) {
+    for (int c = 0; c < cn; c += BK, b ^= 1) {
         const bool more = c + BK < cn;
         if (more) load(c + BK);
         const lds8_t* pt = (const lds8_t*)lds + b * STAGE;
@@ -455,16 +425,11 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product(const ProductArgs a) {
             for (int i = 0; i < FP; i++)
 #pragma unroll
                 for (int j = 0; j < FQ; j++) acc[i][j] = mfma<BF>(pf[i], qf[j], acc[i][j]);
-            if (sums)
-#pragma unroll
-                for (int j = 0; j < FQ; j++) sum[j] = add8<BF>(qf[j], sum[j]);
         }
         if (more) stage(b ^ 1);
         __syncthreads();
     }
 
-    if (sums) store_db<FQ>(a, e, 0, q0 + wq * (BQ / WQ), lane, sum);
-    if (DIR == DW && !a.dw) return;
     store_tile<BF, DIR, FP, FQ, PH>(a, e, 0, p0 + (gated ? wp * (BP / WP / 2) : wp * (BP / WP)), q0 + wq * (BQ / WQ), qn, outs, lane, acc,
                                     (lf32_t*)lds + wave * epilogue_floats<FP, FQ, PH>());
 }
@@ -492,13 +457,13 @@ static __device__ __attribute__((aligned(16))) uint16_t zero_chunk[8];
 //
 // A call with too few tiles to fill the chip gives each tile's contraction to
 // a.split workgroups (k_join adds their sums).
-template <bool BF, int DIR, int BP, int BQ, int WP, int WQ, int S, int BK>
+template <bool BF, int DIR, int BP, int BQ, int WP, int WQ, int S>
 __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs a) {
     constexpr int NT = 64 * WP * WQ, FP = BP / WP / 16, FQ = BQ / WQ / 16;
     static_assert(DIR != FWD || FP % 2 == 0, "SwiGLU's gate and up meet in a wave");
     constexpr bool PC = DIR == FWD, QC = DIR != DW;
-    using PT = typename std::conditional<PC, AlongC<BP, BK>, AcrossC<BP, BK>>::type;
-    using QT = typename std::conditional<QC, AlongC<BQ, BK>, AcrossC<BQ, BK>>::type;
+    using PT = typename std::conditional<PC, AlongC<BP>, AcrossC<BP>>::type;
+    using QT = typename std::conditional<QC, AlongC<BQ>, AcrossC<BQ>>::type;
     constexpr int PS = BP * BK / 8, QS = BQ * BK / 8, NP = PS / NT, NQ = QS / NT, STAGE = (BP + BQ) * 2 * BK;
     static_assert(PS % NT == 0 && QS % NT == 0, "whole chunks per thread");
     static_assert((S - 2) * (NP + NQ) < 64, "loads are counted");
@@ -628,6 +593,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
         for (int j = 0; j < FQ; j++) acc[i][j] = (f32x4)0.0f;
 #pragma unroll
     for (int j = 0; j < FQ; j++) sum[j] = 0.0f;
+    // db: the first tile of p sums the operand that it reads anyway
     const bool sums = DIR == DW && a.db && p0 == 0 && wp == 0;
 
     s16x8 pf[FP], qf[FQ];
@@ -659,7 +625,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
         // p of stage k + 2, in turn.  A wave fetches its part of q of stage k + 1,
         // then of p of stage k + 2, along with its reads of the two halves: a
         // load waits for its turn, which would hold up products behind it.
-        static_assert(BK == 64 && S == 2 && BP == BQ && NP == 4 && NQ == 4, "5 tiles of equal size");
+        static_assert(S == 2 && BP == BQ && NP == 4 && NQ == 4, "5 tiles of equal size");
         constexpr int TILE = BP * 2 * BK;
         const bool second = wave >= 4;
         const int n = (cn - c0 + BK - 1) / BK;
@@ -943,7 +909,7 @@ static Copies copies(const ProductArgs& a, bool fwd, bool dx, bool dw) {
 // the closer the two are; tiles 64 wide read them in shorter rows.  A split pays a second kernel
 // (which has to look groups up) and the parts' way to memory and back: 4 or 7 us
 // and 2.5 TB/s.  Copies pay 3 us and 4 TB/s, which the kernels for any alignment
-// do not need.
+// do not need (dW has none of those).
 // Few rows (k_product_few, forward): W once per 16 rows, 5.2 TB/s (grouped 4.6,
 // and up to 1024 columns 3.9, where workgroups are short), x from the caches at
 // 15 TB/s, or the time of its waves' batches one after another.  In a graph, us: 1 row,
@@ -960,8 +926,8 @@ static Plan plan(const ProductArgs& a, int dir) {
     const Copies c = copies(a, dir == FWD, dir == DX, dir == DW);
     double copy = 0.0;
     if (c.w) copy += 3.0 + 4.0 * E * a.in * a.out / 4e6;
-    if (c.x) copy += 3.0 + 4.0 * a.x_rows * a.in / 4e6;
-    if (c.dz) copy += 3.0 + 4.0 * rows * a.out / 4e6;
+    if (c.x && dir == FWD) copy += 3.0 + 4.0 * a.x_rows * a.in / 4e6;
+    if (c.dz && dir == DX) copy += 3.0 + 4.0 * rows * a.out / 4e6;
     auto row_parts = [&](int bq) { return groups > 1 ? groups * (0.75 + std::max(0.25, per / bq)) : std::ceil(rows / bq); };
 
     Plan best{T128, 1};
@@ -1015,9 +981,10 @@ static int64_t part_bytes(const ProductArgs& a, int dir, int split) {
     return 4 * n * split;
 }
 // db without dw takes one column of x.
-static ProductArgs without_dx(const ProductArgs& a) {
+static ProductArgs only_db(const ProductArgs& a) {
     ProductArgs b = a;
-    if (!b.dw) b.in = 1;
+    b.in = 1;
+    b.dw_f32 = 0;
     return b;
 }
 
@@ -1042,25 +1009,28 @@ int64_t product_workspace(const ProductArgs& a, bool backward) {
         b.dw_f32 = f32;
         part = std::max(part, part_bytes(b, DW, plan(b, DW).split));
     }
-    b.in = 1;
+    b = only_db(a);
     part = std::max(part, part_bytes(b, DW, plan(b, DW).split));
     return layout(a, copies(a, false, tiled(px), true), part).total;
 }
 
-template <int DIR, int BP, int BQ, int WP, int WQ, int S, int KB = 64> static int run(const ProductArgs& a, hipStream_t s) {
+// A launch holds fewer than 2^32 threads.
+static bool too_many(int64_t blocks, int threads) { return blocks > 0xFFFFFFFFll / threads; }
+
+template <int DIR, int BP, int BQ, int WP, int WQ, int S> static int run(const ProductArgs& a, hipStream_t s) {
     const bool gated = DIR == FWD && a.act == WM_ACT_SWIGLU;
     const int outs = columns(a, DIR), cols = gated ? BP / 2 : BP;
     const int64_t qtiles = DIR == DW ? (int64_t)a.E * ((a.out + BQ - 1) / BQ) : row_tiles(a, BQ);
     const int64_t blocks = qtiles * ((outs + cols - 1) / cols) * a.split;
-    if (blocks > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
+    if (too_many(blocks, 64 * WP * WQ)) return (int)hipErrorInvalidConfiguration;
     void (*k)(const ProductArgs);
-    if constexpr (S > 0) k = a.bf16 ? k_product_dma<true, DIR, BP, BQ, WP, WQ, S, KB> : k_product_dma<false, DIR, BP, BQ, WP, WQ, S, KB>;
+    if constexpr (S > 0) k = a.bf16 ? k_product_dma<true, DIR, BP, BQ, WP, WQ, S> : k_product_dma<false, DIR, BP, BQ, WP, WQ, S>;
     else k = a.bf16 ? k_product<true, DIR, BP, BQ, WP, WQ> : k_product<false, DIR, BP, BQ, WP, WQ>;
     hipLaunchKernelGGL(k, dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
     if (a.split > 1) {
         const int64_t rows = DIR == DW ? (int64_t)a.E * a.out : a.rows;
         const int64_t joins = (rows * ((outs + 7) / 8) + 255) / 256;
-        if (joins > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
+        if (too_many(joins, 256)) return (int)hipErrorInvalidConfiguration;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(a.bf16 ? k_join<true, DIR> : k_join<false, DIR>), dim3((uint32_t)joins), dim3(256), 0, s, a);
     }
     return (int)hipGetLastError();
@@ -1092,7 +1062,7 @@ template <int NW> static int run_few(const ProductArgs& a, hipStream_t s) {
     const bool gated = a.act == WM_ACT_SWIGLU;
     const int outs = columns(a, FWD), cols = gated ? 8 : 16;
     const int64_t blocks = row_tiles(a, 16) * ((outs + cols - 1) / cols);
-    if (blocks > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
+    if (too_many(blocks, 64 * NW)) return (int)hipErrorInvalidConfiguration;
     const auto k = a.bf16 ? k_product_few<true, NW> : k_product_few<false, NW>;
     hipLaunchKernelGGL(k, dim3((uint32_t)blocks), dim3(64 * NW), 0, s, a);
     return (int)hipGetLastError();
@@ -1102,7 +1072,7 @@ static int repack(const uint16_t* src, int64_t ld_src, int64_t stride_src, int n
     const int ld = (cols + 7) / 8 * 8;
     const int64_t blocks = ((int64_t)rows * (ld / 8) + 255) / 256;
     if (blocks == 0) return 0;
-    if (blocks > 0x7FFFFFFF || n > 65535) return (int)hipErrorInvalidConfiguration;
+    if (too_many(blocks, 256) || n > 65535) return (int)hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(k_repack, dim3((uint32_t)blocks, n), dim3(256), 0, s, src, ld_src, stride_src, rows, cols, dst, ld, (int64_t)rows * ld);
     return (int)hipGetLastError();
 }
@@ -1156,7 +1126,7 @@ int launch_product_backward(const ProductArgs& args, uint8_t* ws, hipStream_t s)
         if (int rc = run_tiles<DX>(t, px.k, s)) return rc;
     }
     if (dw) {
-        ProductArgs t = without_dx(b);
+        ProductArgs t = b.dw ? b : only_db(b);
         const Plan p = a.rows ? plan(t, DW) : Plan{T128, 1};
         t.split = p.split;
         t.part_db = t.part + (int64_t)p.split * t.E * t.out * t.in;

@@ -19,7 +19,9 @@ inline int64_t size_of(int t) { return t == WM_F32 ? 4 : 2; }
 
 // Sizes are bounded so that row and column indexes stay in 32 bits; element
 // offsets are 64-bit throughout.
-constexpr int kMaxRows = 1 << 30, kMaxDim = 1 << 26, kMaxGroups = 1 << 16;
+constexpr int kMaxRows = 1 << 30, kMaxDim = 1 << 26, kMaxGroups = 65535;
+constexpr int kMaxTokens = (1 << 24) - 1;      // 256 threads for each in one launch
+constexpr int64_t kMaxStride = 1ll << 40, kMaxWeights = 1ll << 48;
 
 // What both directions need; 0 when the descriptor is sound.
 int check_desc(const wm_product_desc* d) {
@@ -31,7 +33,8 @@ int check_desc(const wm_product_desc* d) {
     WM_CHECK_ARG(d->offsets || d->n_groups == 1);
     WM_CHECK_ARG(al(d->offsets, 4) && al(d->token, 4));
     WM_CHECK_ARG(d->token || d->x_rows >= d->rows);
-    WM_CHECK_ARG(d->ldx >= d->in && d->ldw >= d->in);
+    WM_CHECK_ARG(d->ldx >= d->in && d->ldw >= d->in && d->ldx <= kMaxStride && d->ldw <= kMaxStride);
+    WM_CHECK_ARG((int64_t)d->in * d->out <= kMaxWeights / d->n_groups);
     WM_CHECK_ARG(d->n_groups == 1 || d->w_stride >= (int64_t)(d->out - 1) * d->ldw + d->in);
     WM_CHECK_ARG(d->act >= WM_ACT_NONE && d->act <= WM_ACT_SIGMOID);
     return WM_OK;
@@ -176,7 +179,7 @@ extern "C" int wm_combine_rows(int dtype, const void* y, int64_t ld_y, int rows,
                                int T, int K, int H, const void* residual, int64_t ld_residual, void* out,
                                int64_t ld_out, int out_type, void* stream) {
     WM_CHECK_ARG(dtype_ok(dtype) && (out_type == dtype || out_type == WM_F32));
-    WM_CHECK_ARG(T >= 0 && K >= 0 && rows >= 0 && H >= 1 && H <= kMaxDim && (int64_t)T * K <= 0x7FFFFFFF);
+    WM_CHECK_ARG(T >= 0 && T <= kMaxTokens && K >= 0 && rows >= 0 && H >= 1 && H <= kMaxDim && (int64_t)T * K <= 0x7FFFFFFF);
     if (T == 0) return WM_OK;
     WM_CHECK_ARG(out && al(out, size_of(out_type)) && ld_out >= H);
     WM_CHECK_ARG(K == 0 || (row && al(row, 4) && al(w, 4)));
@@ -207,6 +210,7 @@ extern "C" int wm_combine_rows_backward(int dtype, const void* dout, int64_t ld_
                                         int H, void* dy, int64_t ld_dy, float* dw, void* stream) {
     WM_CHECK_ARG(dtype_ok(dtype) && (dout_type == dtype || dout_type == WM_F32));
     WM_CHECK_ARG(T >= 0 && K >= 0 && rows >= 0 && H >= 1 && H <= kMaxDim && (int64_t)T * K <= 0x7FFFFFFF);
+    WM_CHECK_ARG((int64_t)T * ((K + 4ll) / 5) <= kMaxTokens / 2);
     if (T == 0 || K == 0 || (!dy && !dw)) return WM_OK;
     WM_CHECK_ARG(dout && al(dout, size_of(dout_type)) && ld_dout >= H);
     WM_CHECK_ARG(row && al(row, 4) && al(w, 4) && al(dw, 4));

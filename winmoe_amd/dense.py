@@ -72,10 +72,16 @@ def _dense(t: torch.Tensor, shape, dtype, name: str) -> int:
 
 
 def _new(like: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
-    """An output or workspace for work on `stream` (None: the current stream)."""
-    t = like.new_empty(shape, dtype=dtype)
-    if stream is not None:
-        t.record_stream(stream)
+    """An output or workspace for work on `stream` (None: the current stream).
+
+    Memory freed on the current stream may still be in use there, so what another
+    stream writes comes from that stream's own; it is kept from reuse until the
+    current stream, where the result may be read, is done with it."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        t = like.new_empty(shape, dtype=dtype)
+    t.record_stream(torch.cuda.current_stream())
     return t
 
 
