@@ -120,6 +120,28 @@ WM_DEV TileId tile_id(int block, int blocks, int nP) {
     const int qb = t / (TILE_ROWS * nP), nq = min(TILE_ROWS, blocks / nP - TILE_ROWS * qb), in = t - qb * TILE_ROWS * nP;
     return {in / nq, TILE_ROWS * qb + in % nq};
 }
+// Grouped products: how much work a row tile holds is not known on the host (the
+// last ones hold none, an expert's dW takes as long as its rows), so blocks of
+// `g` row tiles times all column tiles go round the XCDs in turn, the rest in
+// blocks of one, then in runs as above.  16384 rows of 64 experts' 1024 x 2048,
+// the popular experts first, in runs and in turn: dx 157 and 125 us (256 x 256
+// tiles), dW 242 and 186 us; 4004 rows forward 72 and 60 us.
+WM_DEV TileId tile_id_grouped(int block, int blocks, int nP, int g) {
+    int q0 = 0;
+#pragma unroll
+    for (int level = 0; level < 2; level++) {
+        const int n = level ? 1 : g, per = n * nP, rounds = blocks / (8 * per), full = rounds * 8 * per;
+        if (block < full) {
+            const int i = block / 8, in = i % per;
+            return {in / n, q0 + n * (i / per * 8 + block % 8) + in % n};
+        }
+        block -= full;
+        blocks -= full;
+        q0 += rounds * 8 * n;
+    }
+    const TileId t = tile_id(block, blocks, nP);
+    return {t.p, q0 + t.q};
+}
 
 // ------------------------------------------------------------------ LDS tiles
 
@@ -458,6 +480,10 @@ static __device__ __attribute__((aligned(16))) uint16_t zero_chunk[8];
 // A call with too few tiles to fill the chip gives each tile's contraction to
 // a.split workgroups (k_join adds their sums).
 //
+// 128 wide tiles have 8 waves: a wave's loads are issued one behind the other
+// before its products, and with 4 waves each issues twice as many (2048 x 2048 x
+// 2048: 31.9 and 28.6 us forward, 36.7 and 31.3 us for dW).
+//
 // Grouped products of few rows per expert are bound by memory: 5120 rows of 512
 // experts' 4096 x 1024 take 790 us, 5.5 TB/s.  dx of 16384 rows of 64 experts'
 // 1024 x 2048 takes 160 us (128 x 128 tiles, 430 TFLOP/s), dW 185 us.
@@ -472,7 +498,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
     static_assert(PS % NT == 0 && QS % NT == 0, "whole chunks per thread");
     static_assert((S - 2) * (NP + NQ) < 64, "loads are counted");
     constexpr int PH = WP * WQ * 4 * epilogue_floats<FP, FQ, 1>() > 160 * 1024 ? 2 : 1, EPI = WP * WQ * 4 * epilogue_floats<FP, FQ, PH>();
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[NT == 512 && DIR != DW ? STAGE / 2 * 5 : S * STAGE > EPI ? S * STAGE : EPI];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[BP == 256 && DIR != DW ? STAGE / 2 * 5 : S * STAGE > EPI ? S * STAGE : EPI];
     static_assert(sizeof(lds) >= EPI, "the epilogue fits");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -482,7 +508,8 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
     const int cols = gated ? BP / 2 : BP;
     const int nP = (outs + cols - 1) / cols;
     const int tiles = gridDim.x / a.split, part = blockIdx.x / tiles;
-    const TileId id = tile_id(blockIdx.x % tiles, tiles, nP);
+    const TileId id = a.offsets ? tile_id_grouped(blockIdx.x % tiles, tiles, nP, DIR == DW ? (a.out + BQ - 1) / BQ : TILE_ROWS)
+                                : tile_id(blockIdx.x % tiles, tiles, nP);
     const int p0 = id.p * cols;
     int e, q0, qn, c0 = 0, cn;
     const uint16_t* w = nullptr;
@@ -617,7 +644,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
             for (int j = 0; j < FQ; j++) sum[j] = add8<BF>(qf[j], sum[j]);
     };
 
-    if constexpr (NT == 512 && DIR != DW) {
+    if constexpr (BP == 256 && DIR != DW) {
         // Two groups of 4 waves, one of each group per SIMD, take turns: while
         // one reads its operands of half a stage the other one multiplies.  Time
         // runs in slots that end in a barrier: group 0 reads the halves of stage
@@ -878,7 +905,7 @@ struct TileCost {
     float alone, share, ends;
 };
 static constexpr TileCost kTiles[] = {
-    {T256, 256, 256, 1, 1.40f, 1.65f, 6.0f},  {T128, 128, 128, 2, 0.82f, 0.54f, 3.0f}, {T128x64, 128, 64, 2, 0.58f, 0.36f, 2.5f},
+    {T256, 256, 256, 1, 1.40f, 1.60f, 6.0f},  {T128, 128, 128, 2, 0.73f, 0.52f, 3.0f}, {T128x64, 128, 64, 2, 0.50f, 0.35f, 2.5f},
     {T128x32, 128, 32, 2, 0.40f, 0.33f, 2.0f}, {T64, 64, 64, 2, 0.40f, 0.27f, 2.0f},    {T64x32, 64, 32, 3, 0.34f, 0.20f, 2.0f},
     {T64x16, 64, 16, 4, 0.34f, 0.15f, 2.0f},   {ANY128, 128, 128, 2, 1.00f, 0.69f, 3.0f}, {ANY32, 128, 32, 4, 0.70f, 0.45f, 2.0f},
 };
@@ -914,7 +941,9 @@ static Copies copies(const ProductArgs& a, bool fwd, bool dx, bool dw) {
 // The kernel and the number of parts with the least estimated time.  The chip
 // is taken as 256 CUs.  The host does not know the groups: rows are taken as
 // spread evenly at random over the experts, with some more tiles than that
-// makes, as groups are skewed.
+// makes, as groups are skewed; smaller tiles, which fetch more, share a CU less
+// well there than in one group (dx of 32768 rows of 128 experts' 1024 x 1024: 256
+// x 256 124 us, 128 x 128 141 us; in one group their estimates hold).
 //
 // Tiles: reading the weights (writing, for dW) overlaps the products, the worse
 // the closer the two are; tiles 64 wide read them in shorter rows.  A split pays a second kernel
@@ -951,7 +980,8 @@ static Plan plan(const ProductArgs& a, int dir) {
         for (int s = 1; s <= (any ? 1 : 16) && s * 2 <= stages + 1; s *= 2) {
             if (s > 1 && s * sums > 512e6) break;
             const double n = std::ceil(p * q * s / 256), turns = std::max(1.0, n / t.resident);
-            const double work = std::ceil(stages / s) * std::max(t.alone * turns, t.share * n) + t.ends * turns;
+            const double share = groups > 1 && t.resident > 1 ? 1.25 * t.share : t.share;
+            const double work = std::ceil(stages / s) * std::max(t.alone * turns, share * n) + t.ends * turns;
             const double stream = t.bp < 128 ? 1.15 * memory : memory;
             const double more = std::max(work, stream), less = std::min(work, stream);
             const double us = 3.0 + more + 0.35 * less * (less / more) * (less / more) + (any ? 0.0 : copy) +
@@ -1050,13 +1080,13 @@ template <int DIR, int BP, int BQ, int WP, int WQ, int S> static int run(const P
 template <int DIR> static int run_tiles(const ProductArgs& a, Kernel k, hipStream_t s) {
     switch (k) {
     case T256: return run<DIR, 256, 256, 2, 4, 2>(a, s);
-    case T128: return run<DIR, 128, 128, 2, 2, 2>(a, s);
+    case T128: return run<DIR, 128, 128, 2, 4, 2>(a, s);
     case T64: return run<DIR, 64, 64, 2, 2, 4>(a, s);
     default: break;
     }
     if constexpr (DIR != DW) {
         switch (k) {
-        case T128x64: return run<DIR, 128, 64, 2, 2, 3>(a, s);
+        case T128x64: return run<DIR, 128, 64, 4, 2, 3>(a, s);
         case T128x32: return run<DIR, 128, 32, 4, 1, 4>(a, s);
         case T64x32: return run<DIR, 64, 32, 2, 2, 4>(a, s);
         case T64x16: return run<DIR, 64, 16, 2, 1, 4>(a, s);
