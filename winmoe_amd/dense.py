@@ -38,12 +38,16 @@ _DESC = struct.Struct("8i16q")
 # Checks cost the host a few microseconds a call, so they are plain Python on
 # what a tensor hands out at once.
 
-def _dev(t: torch.Tensor, name: str) -> torch.Tensor:
+# The current device's number (torch.cuda.current_device() initialises first,
+# 0.2 us; whoever holds a device tensor has done that).
+_current = torch._C._cuda_getDevice
+
+
+def _dev(t: torch.Tensor, name: str) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA (HIP) tensor")
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, not on the current device cuda:{torch.cuda.current_device()}")
-    return t
+    if t.get_device() != _current():
+        raise ValueError(f"{name} is on {t.device}, not on the current device cuda:{_current()}")
 
 
 def _rows(t: torch.Tensor, rows: int, cols: int, dtype, name: str) -> int:
@@ -51,9 +55,13 @@ def _rows(t: torch.Tensor, rows: int, cols: int, dtype, name: str) -> int:
     _dev(t, name)
     if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    shape, strides = t.shape, t.stride()
-    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
-        raise ValueError(f"{name} must be {[rows, cols]}, got {list(shape)}")
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name} must be {[rows, cols]}, got {list(t.shape)}")
+    return _distance(t, rows, cols, name)
+
+
+def _distance(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
+    strides = t.stride()
     if (cols > 1 and strides[1] != 1) or (rows > 1 and strides[0] < cols):
         raise ValueError(f"{name} must have contiguous rows, got strides {strides}")
     return strides[0] if rows > 1 else max(cols, 1)         # a single row's stride means nothing
@@ -91,9 +99,10 @@ def _raw(stream, t: torch.Tensor) -> int:
 
 def _dtype16(t: torch.Tensor, name: str):
     _dev(t, name)
-    if t.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{name} must be float16 or bfloat16, got {t.dtype}")
-    return t.dtype
+    dt = t.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise ValueError(f"{name} must be float16 or bfloat16, got {dt}")
+    return dt
 
 
 def _act(act: str) -> int:
@@ -112,8 +121,11 @@ def _out_type(dtype, like, name: str):
 def _operands(x, w, offsets, token):
     """(rows, in, out, E, x rows, offsets, token, x, ldx, w, ldw, w stride) of a product:
     w [E][out][in], or [out][in] when offsets is None."""
-    dt = _dtype16(x, "x")
+    _dev(x, "x")
     _dev(w, "w")
+    dt = x.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise ValueError(f"x must be float16 or bfloat16, got {dt}")
     shape, strides = w.shape, w.stride()
     if offsets is None:
         if len(shape) != 2:
@@ -136,10 +148,10 @@ def _operands(x, w, offsets, token):
     stride = w.stride(0) if E > 1 else 0
     if E > 1 and stride < (out - 1) * ldw + inn:
         raise ValueError(f"the experts of w overlap: strides {w.stride()}")
-    if x.dim() != 2:
+    if x.dim() != 2 or x.shape[1] != inn:
         raise ValueError(f"x must be [rows][{inn}], got {list(x.shape)}")
     x_rows = x.shape[0]
-    ldx = _rows(x, x_rows, inn, dt, "x")
+    ldx = _distance(x, x_rows, inn, "x")
     rows, tok = x_rows, 0
     if token is not None:
         rows = token.numel()
@@ -242,16 +254,17 @@ class Grouping(NamedTuple):
 
 def group_by_expert(ids: torch.Tensor, E: int, stream=None) -> Grouping:
     """Sorts the picks ids int32 [T][K] by expert, stably.  A pick outside [0, E) (padding) belongs to none."""
-    _dev(ids, "ids")
-    if ids.dim() != 2 or ids.shape[1] < 1:
-        raise ValueError(f"ids must be [T][K], got {list(ids.shape)}")
-    p = _dense(ids, ids.shape, torch.int32, "ids")
+    shape = ids.shape if isinstance(ids, torch.Tensor) else ()
+    p = _dense(ids, shape, torch.int32, "ids")
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"ids must be [T][K], got {list(shape)}")
     if E < 1:
         raise ValueError("there must be an expert")
-    T, K = ids.shape
-    g = Grouping(*(_new(ids, s, torch.int32, stream) for s in ((E + 1,), (T * K,), (T, K))))
-    check(load().wm_group_by_expert(p, T, K, E, *(t.data_ptr() for t in g), _raw(stream, ids)), "wm_group_by_expert")
-    return g
+    T, K = shape
+    offsets, token, row = _new(ids, (E + 1,), torch.int32, stream), _new(ids, (T * K,), torch.int32, stream), _new(ids, shape, torch.int32, stream)
+    check(load().wm_group_by_expert(p, T, K, E, offsets.data_ptr(), token.data_ptr(), row.data_ptr(), _raw(stream, ids)),
+          "wm_group_by_expert")
+    return Grouping(offsets, token, row)
 
 
 def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, token: Optional[torch.Tensor] = None,
@@ -296,16 +309,17 @@ def act_backward(dy: torch.Tensor, pre: torch.Tensor, act: str, out: Optional[to
 
 def _combine_args(y, row, w):
     """(type, T, K, H, distance of y's rows, row, w)."""
-    dt = _dtype16(y, "y")
-    if y.dim() != 2 or y.shape[1] < 1:
-        raise ValueError(f"y must be [rows][H], got {list(y.shape)}")
-    ldy = _rows(y, *y.shape, dt, "y")
-    _dev(row, "row")
-    if row.dim() != 2:
-        raise ValueError(f"row must be [T][K], got {list(row.shape)}")
-    rp = _dense(row, row.shape, torch.int32, "row")
-    wp = 0 if w is None else _dense(w, row.shape, torch.float32, "w")
-    return dt, row.shape[0], row.shape[1], y.shape[1], ldy, rp, wp
+    dt, shape = _dtype16(y, "y"), y.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"y must be [rows][H], got {list(shape)}")
+    rows, H = shape
+    ldy = _distance(y, rows, H, "y")
+    shape = row.shape if isinstance(row, torch.Tensor) else ()
+    rp = _dense(row, shape, torch.int32, "row")
+    if len(shape) != 2:
+        raise ValueError(f"row must be [T][K], got {list(shape)}")
+    wp = 0 if w is None else _dense(w, shape, torch.float32, "w")
+    return dt, shape[0], shape[1], H, ldy, rp, wp
 
 
 def combine(y: torch.Tensor, row: torch.Tensor, w: Optional[torch.Tensor] = None,
