@@ -486,7 +486,7 @@ static __device__ __attribute__((aligned(16))) uint16_t zero_chunk[8];
 //
 // Grouped products of few rows per expert are bound by memory: 5120 rows of 512
 // experts' 4096 x 1024 take 790 us, 5.5 TB/s.  dx of 16384 rows of 64 experts'
-// 1024 x 2048 takes 160 us (128 x 128 tiles, 430 TFLOP/s), dW 185 us.
+// 1024 x 2048 takes 125 to 132 us (256 x 256 tiles, 520 TFLOP/s), dW 186 to 192 us.
 template <bool BF, int DIR, int BP, int BQ, int WP, int WQ, int S>
 __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs a) {
     constexpr int NT = 64 * WP * WQ, FP = BP / WP / 16, FQ = BQ / WQ / 16;
@@ -658,10 +658,11 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_product_dma(const ProductArgs 
         // load waits for its turn, which would hold up products behind it.
         //
         // 4096 x 16384 x 4096 takes 435 to 470 us (1170 to 1260 TFLOP/s; a library
-        // product 1460).  A stage takes 1.6 us of which the matrix instructions
-        // need 0.9 to 1.2: LDS bandwidth, 64 KB written and 192 KB read per stage,
-        // bounds it.  4 waves of 128 x 128,
-        // which read a third less, 477 us, as their sums move between register files.
+        // product 1460).  A stage takes 1.5 to 1.6 us; its matrix instructions need
+        // 0.9 us, 1.2 at the clock that long products run at, its 192 KB of LDS
+        // reads 0.6 at the 315 B/ns that a CU reaches, its 64 KB of loads 0.5 from
+        // L2 (120 B/ns).  4 waves of 128 x 128, which read a third less, took 477 us,
+        // as their sums move between register files.
         static_assert(S == 2 && BP == BQ && NP == 4 && NQ == 4, "5 tiles of equal size");
         constexpr int TILE = BP * 2 * BK;
         const bool second = wave >= 4;
