@@ -497,6 +497,59 @@ def chain(dense, x, ids, p, gu, down, E, T, K):
     return g, pre, h, y, dense.combine(y, g.row, p, residual=x)
 
 
+@pytest.mark.parametrize("size", [(1, 2056, 520), (17, 4096, 8200), (130, 4096, 520), (3000, 200, 4104), (50, 71, 57), (700, 4096, 136)],
+                         ids=str)
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+def test_residual_in_place(dense, size, act):
+    """residual may be the result: whole tiles, parts joined afterwards and few rows give the bits of a result of its own."""
+    T, K, N = size
+    x, w, b = rnd(91, T, K), rnd(92, 2 * N, K, scale=0.1), rnd(93, 2 * N)
+    cols = N if act == "swiglu" else 2 * N
+    res = rnd(94, T, cols + 24)[:, :cols]
+    pre = torch.empty(T, 2 * N, dtype=x.dtype, device="cuda")
+    want = dense.linear(x, w, bias=b, act=act, residual=res, pre=pre)
+    again = torch.empty_like(pre)
+    got = dense.linear(x, w, bias=b, act=act, residual=res, out=res, pre=again)
+    assert got is res and torch.equal(got, want) and torch.equal(again, pre)
+
+
+def test_activation_gradient_in_place(dense):
+    """dz may be pre, for wide and narrow rows alike."""
+    for T, n in ((5, 1001), (300, 512)):
+        for act in ("gelu", "swiglu"):
+            pre, dy = rnd(95, T, 2 * n if act == "swiglu" else n), rnd(96, T, n)
+            want = dense.act_backward(dy, pre, act)
+            assert torch.equal(dense.act_backward(dy, pre, act, out=pre), want)
+
+
+def test_combine_residual_in_place(dense):
+    y, p, res = rnd(97, 70, 1001), torch.rand(23, 3, device="cuda"), rnd(98, 23, 1001)
+    row = torch.randint(-1, 70, (23, 3), dtype=torch.int32, device="cuda")
+    want = dense.combine(y, row, p, residual=res)
+    assert torch.equal(dense.combine(y, row, p, residual=res, out=res), want)
+
+
+def test_popular_experts_first(dense):
+    """Groups of very different sizes in descending order, some empty: every tile of every group is computed once."""
+    sizes = [700, 260, 257, 256, 130, 129, 64, 33, 16, 5, 1, 0, 0, 1, 0, 40, 0, 3, 0]
+    E, H, N, R = len(sizes), 264, 520, sum(sizes) + 7
+    off = torch.tensor([0] + sizes).cumsum(0).int().cuda()
+    x, w, dz = rnd(99, R, H), rnd(100, E, N, H, scale=0.1), rnd(101, R, N)
+    y, dx = torch.full((R, N), 7.0, dtype=x.dtype, device="cuda"), torch.full((R, H), 7.0, dtype=x.dtype, device="cuda")
+    dense.grouped_matmul(x, w, off, out=y)
+    _, dw, _ = dense.grouped_matmul_backward(dz, x, w, off, dx=dx, dw_dtype=torch.float32)
+    assert bool((y[-7:] == 7).all()) and bool((dx[-7:] == 7).all())
+    at = 0
+    for e, n in enumerate(sizes):
+        r = slice(at, at + n)
+        X, W, Z = x[r].double(), w[e].double(), dz[r].double()
+        # a result's rounding to bf16, and its fp32 sum of up to 700 products in any order
+        for got, want, size, half in ((y[r], X @ W.T, X.abs() @ W.abs().T, 2.0 ** -8), (dx[r], Z @ W, Z.abs() @ W.abs(), 2.0 ** -8),
+                                      (dw[e], Z.T @ X, Z.abs().T @ X.abs(), 0.0)):
+            assert bool(((got.double() - want).abs() <= half * want.abs() + 1.01 * 700 * 2.0 ** -24 * size).all()), e
+        at += n
+
+
 def test_on_another_stream(dense):
     x, w = rnd(62, 300, 512), rnd(63, 384, 512, scale=0.1)
     want = dense.linear(x, w, act="silu")
