@@ -203,8 +203,10 @@ def _product_backward(dz, x, w, offsets, token, need_dx, need_dw, need_db, dw_dt
     dxp = lddx = dwp = dbp = 0
     if need_dx or dx is not None:
         if dx is None:
-            dx = _new(x, (rows, inn), dt, stream)
-        dxp, lddx = dx.data_ptr(), _rows(dx, rows, inn, dt, "dx")
+            dx, lddx = _new(x, (rows, inn), dt, stream), inn
+        else:
+            lddx = _rows(dx, rows, inn, dt, "dx")
+        dxp = dx.data_ptr()
     if need_dw or dw is not None:
         if dw is None:
             dw = _new(x, w.shape, wt, stream)
@@ -300,8 +302,10 @@ def act_backward(dy: torch.Tensor, pre: torch.Tensor, act: str, out: Optional[to
     T, n = dy.shape
     wide = 2 * n if act == "swiglu" else n
     ldy, ldp = _rows(dy, T, n, dt, "dy"), _rows(pre, T, wide, dt, "pre")
-    dz = _new(pre, (T, wide), dt, stream) if out is None else out
-    ldz = _rows(dz, T, wide, dt, "out")
+    if out is None:
+        dz, ldz = _new(pre, (T, wide), dt, stream), wide
+    else:
+        dz, ldz = out, _rows(out, T, wide, dt, "out")
     check(load().wm_act_backward(_TYPES[dt], a, T, n, dy.data_ptr(), ldy, pre.data_ptr(), ldp, dz.data_ptr(), ldz,
                                  _raw(stream, pre)), "wm_act_backward")
     return dz
@@ -334,8 +338,10 @@ def combine(y: torch.Tensor, row: torch.Tensor, w: Optional[torch.Tensor] = None
     if out_dtype is None and (out is not None or residual is not None):
         out_dtype = (residual if out is None else out).dtype
     ot = _out_type(out_dtype, dt, "out_dtype")
-    o = _new(y, (T, H), ot, stream) if out is None else out
-    ldo = _rows(o, T, H, ot, "out")
+    if out is None:
+        o, ldo = _new(y, (T, H), ot, stream), H
+    else:
+        o, ldo = out, _rows(out, T, H, ot, "out")
     sp = ldr = 0
     if residual is not None:
         sp, ldr = residual.data_ptr(), _rows(residual, T, H, ot, "residual")
