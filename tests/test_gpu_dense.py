@@ -562,6 +562,14 @@ def test_on_another_stream(dense):
     assert torch.equal(got, want) and torch.equal(also, want)
 
 
+def test_a_stream_of_another_device_is_refused(dense):
+    from types import SimpleNamespace
+    x, w = rnd(62, 5, 64), rnd(63, 24, 64)
+    out = torch.empty(5, 24, dtype=x.dtype, device="cuda")
+    with pytest.raises(ValueError, match="stream"):
+        dense.linear(x, w, out=out, stream=SimpleNamespace(cuda_stream=0, device_index=x.get_device() + 1))
+
+
 def test_memory_of_the_current_stream_is_not_written_on_another(dense):
     """What a call on another stream writes does not lie where the current stream may still be reading."""
     x, w = rnd(62, 300, 512), rnd(63, 384, 512, scale=0.1)

@@ -94,7 +94,11 @@ def _new(like: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
 
 
 def _raw(stream, t: torch.Tensor) -> int:
-    return torch._C._cuda_getCurrentRawStream(t.get_device()) if stream is None else stream.cuda_stream
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(t.get_device())
+    if stream.device_index != t.get_device():
+        raise ValueError(f"the stream is on device {stream.device_index}, the tensors on {t.get_device()}")
+    return stream.cuda_stream
 
 
 def _dtype16(t: torch.Tensor, name: str):
