@@ -96,7 +96,8 @@ KERNEL_SHAPES = {
            (4000, 264, 136, 1), (17, 4096, 8200, 1), (130, 4096, 520, 3), (4000, 1032, 8200, 9),
            (2000, 4096, 57, 3), (50, 264, 16, 3), (2000, 4096, 57, 64), (700, 4096, 136, 1), (700,
            4096, 136, 3), (2000, 71, 2056, 1), (2000, 71, 2056, 3), (700, 71, 2056, 1), (130, 71,
-           2056, 3), (2000, 264, 136, 64), (700, 4096, 136, 9)],
+           2056, 3), (2000, 264, 136, 64), (700, 4096, 136, 9),
+           (50, 4096, 2056, 3)],
     "dx": [(3000, 2056, 72, 1), (4000, 1032, 136, 9), (4000, 2056, 200, 9), (3000, 4104, 136, 1), (2000, 520, 8200, 1),
            (2000, 520, 8200, 3), (260, 4104, 72, 9), (3, 2056, 8200, 1), (130, 264, 4104, 9), (4000, 520, 72, 1),
            (4000, 520, 72, 3), (3000, 136, 4104, 1), (2000, 72, 8200, 9), (16, 4104, 72, 9), (1, 2056, 2056, 1),
@@ -104,7 +105,8 @@ KERNEL_SHAPES = {
            (2000, 520, 72, 3), (1000, 72, 2056, 1), (1000, 72, 2056, 3), (50, 71, 57, 3), (700, 71, 57, 1),
            (130, 200, 4104, 9), (3000, 4104, 136, 3),
            (2000, 264, 136, 1), (700, 71, 2056, 3), (700, 64, 8200, 1), (700, 64, 8200, 3), (4000,
-           1032, 57, 1), (4000, 1032, 57, 3), (700, 71, 2056, 9), (700, 71, 8200, 3), (2000, 1032, 8200, 3)],
+           1032, 57, 1), (4000, 1032, 57, 3), (700, 71, 2056, 9), (700, 71, 8200, 3), (2000, 1032, 8200, 3),
+           (1, 4096, 2056, 1), (50, 1032, 8200, 3)],
     "dw": [(200, 4104, 520, 1), (300, 4104, 24, 9), (4000, 72, 8200, 1), (130, 2056, 8200, 1), (700, 1032, 1032, 9),
            (70, 72, 24, 1), (70, 72, 24, 3), (1000, 72, 24, 1), (4000, 72, 24, 3), (1000, 71, 57, 1), (130, 264, 8200, 1),
            (700, 4096, 2056, 3)],

@@ -906,8 +906,8 @@ struct TileCost {
     float alone, share, ends;
 };
 static constexpr TileCost kTiles[] = {
-    {T256, 256, 256, 1, 1.40f, 1.60f, 6.0f},  {T128, 128, 128, 2, 0.73f, 0.52f, 3.0f}, {T128x64, 128, 64, 2, 0.50f, 0.35f, 2.5f},
-    {T128x32, 128, 32, 2, 0.40f, 0.33f, 2.0f}, {T64, 64, 64, 2, 0.40f, 0.27f, 2.0f},    {T64x32, 64, 32, 3, 0.34f, 0.20f, 2.0f},
+    {T256, 256, 256, 1, 1.40f, 1.60f, 6.0f},  {T128, 128, 128, 2, 0.73f, 0.52f, 3.0f}, {T128x64, 128, 64, 2, 0.54f, 0.35f, 2.5f},
+    {T128x32, 128, 32, 2, 0.42f, 0.33f, 2.0f}, {T64, 64, 64, 2, 0.37f, 0.24f, 2.0f},    {T64x32, 64, 32, 3, 0.34f, 0.20f, 2.0f},
     {T64x16, 64, 16, 4, 0.34f, 0.15f, 2.0f},   {ANY128, 128, 128, 2, 1.00f, 0.69f, 3.0f}, {ANY32, 128, 32, 4, 0.70f, 0.45f, 2.0f},
 };
 struct Plan {
